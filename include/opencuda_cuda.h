@@ -214,6 +214,96 @@ int oc_sdpa_workspace_size(int seq_len, size_t *bytes);
 int oc_sdpa(const float *q, const float *k, const float *v, float *o, int seq_len, int head_dim, void *workspace,
             size_t workspace_bytes, void *stream);
 
+/* ---- paged key/value cache (no counterpart in the reference, whose cache is
+ * one growing Vec per head, KvCacheHead llm:530-596) -----------------------
+ * Keys and values of many sequences in pages of page_size tokens,
+ * [num_layers][num_pages][kv_heads][page_size][head_dim] each.  Sequence s
+ * holds seq_len[s] tokens; token t sits in page page_table[s][t / page_size]
+ * at offset t % page_size.  refcount[p] counts the sequences that hold page p
+ * (0 = free); a page that two sequences share is full, so it is never
+ * written.  All arrays are device memory of the caller; a fresh cache has
+ * page_table -1, seq_len, refcount and status 0, and pools without NaN (zeros).  page_size is a power of
+ * two up to 1024, head_dim at most 256.
+ *
+ * The operations run on the device in stream order and can be captured into
+ * CUDA graphs; calls that touch one cache must be ordered by the caller (they
+ * change it, and use its scratch).  Contents of device arrays (ids, offsets,
+ * lengths) cannot be checked by the host: a kernel that meets a bad one sets
+ * a bit of *status and stays inside the arrays.  extend, fork and copy_pages
+ * then change nothing at all; the others skip the entry. */
+#define OC_KV_F32 0
+#define OC_KV_F16 1
+#define OC_KV_BF16 2
+#define OC_KV_NO_PAGES 1     /* too few free pages */
+#define OC_KV_BAD_SEQUENCE 2 /* an id outside the table, one used twice, or a child that is not empty */
+#define OC_KV_ROW_FULL 4     /* more tokens than a row of the page table holds */
+#define OC_KV_BAD_PAGE 8     /* a page number outside the pool, or a token without a page */
+typedef struct {
+  void *k, *v;         /* [num_layers][num_pages][kv_heads][page_size][head_dim] */
+  int32_t *page_table; /* [max_seqs][max_pages_per_seq] */
+  int32_t *seq_len;    /* [max_seqs] */
+  int32_t *refcount;   /* [num_pages] */
+  int32_t *status;     /* [1] OC_KV_* bits, set by kernels, cleared by the caller */
+  int32_t *scratch;    /* oc_kv_scratch_size bytes, for extend, fork, compact and copy_pages */
+  int dtype;           /* OC_KV_F32, OC_KV_F16 or OC_KV_BF16 */
+  int num_layers, num_pages, kv_heads, page_size, head_dim, max_seqs, max_pages_per_seq;
+} oc_kv_cache;
+
+/* Bytes of oc_kv_cache.scratch (num_pages <= 2^20, max_seqs <= 2^18). */
+int oc_kv_scratch_size(int num_pages, int max_seqs, size_t *bytes);
+/* Sequence seqs[i] grows by counts[i] >= 0 tokens: seq_len += counts[i], and
+ * the pages it lacks are taken from the free ones, lowest number first, in
+ * the order of the list.  Each sequence at most once. */
+int oc_kv_extend(const oc_kv_cache *cache, const int32_t *seqs, const int32_t *counts, int n, void *stream);
+/* children[i] (empty, each at most once, none of them a parent) becomes a
+ * copy of parents[i]: the full pages are shared, a last page that is partly
+ * filled is copied, over all layers, to a free page (lowest first, in the
+ * order of the list). */
+int oc_kv_fork(const oc_kv_cache *cache, const int32_t *parents, const int32_t *children, int n, void *stream);
+/* The sequences' pages lose a holder each, their rows and lengths are
+ * cleared.  An id given twice, or a sequence that is empty already, is freed
+ * once. */
+int oc_kv_free(const oc_kv_cache *cache, const int32_t *seqs, int n, void *stream);
+/* The L pages in use end up as pages 0 .. L - 1: the i-th page in use from
+ * number L on moves, over all layers, to the i-th free one below L; rows and
+ * counts follow. */
+int oc_kv_compact(const oc_kv_cache *cache, void *stream);
+/* Page dst[i] := page src[i] over all layers, keys and values; tables and
+ * counts stay.  No page may be written twice, or written and read. */
+int oc_kv_copy_pages(const oc_kv_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream);
+/* Writes the new tokens' keys and values to their pages of one layer, and
+ * prepares the queries.  The call names n sequences: entry b is sequence
+ * seqs[b] (seqs NULL: b) with new tokens cu[b] .. cu[b + 1] - 1 of `tokens`
+ * (cu NULL: n = tokens, one token each), which are its last ones: seq_len
+ * counts them already (oc_kv_extend).  q [tokens][q_heads][head_dim], k and v
+ * [tokens][kv_heads][head_dim] in the cache's type, token strides in elements
+ * (heads of a token are contiguous).  In f32, rounded once at the end:
+ *   x := x / sqrt(mean(x^2) + eps) * weight   (q_weight / k_weight [head_dim]
+ *        in the cache's type; NULL: no norm)
+ *   the first rot_dim features are rotated by position * inv_freq[j]
+ *        (inv_freq [rot_dim / 2] f32, the angle in f64): pairs (j, j +
+ *        rot_dim / 2), or (2j, 2j + 1) when interleaved; rot_dim 0: none.
+ * q_out [tokens][q_heads][head_dim] may be q itself; q_heads 0: keys and
+ * values alone.  Rows of tokens behind the last sequence stay as they are. */
+int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const int32_t *cu, const int32_t *seqs,
+                 int q_heads, const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                 int64_t v_stride, void *q_out, int64_t q_out_stride, const void *q_weight, const void *k_weight,
+                 float eps, const float *inv_freq, int rot_dim, int interleaved, void *stream);
+/* Attention of the new tokens over their sequences' pages of one layer (the
+ * batch as for oc_kv_append, queries with norms and rotation done):
+ *   out = softmax(scale * q . K^T) . V
+ * query head h reads kv head h / (q_heads / kv_heads).  A token at position p
+ * sees keys j < seq_len with j <= p when causal and j > p - window when
+ * window > 0; a row that sees none gives 0, and what a row does not see has
+ * no part in it, whatever it holds.  f32 accumulation and softmax statistics.
+ * workspace: oc_kv_attention_workspace_size bytes, for partial results of
+ * long sequences that several blocks share; calls that may overlap need one
+ * each. */
+int oc_kv_attention_workspace_size(const oc_kv_cache *cache, int tokens, int n, int q_heads, size_t *bytes);
+int oc_kv_attention(const oc_kv_cache *cache, int layer, int tokens, int n, const int32_t *cu, const int32_t *seqs,
+                    int q_heads, const void *q, int64_t q_stride, void *out, int64_t out_stride, float scale,
+                    int causal, int window, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- MLA low-rank KV projections (blas:1045-1078) ----------------------- */
 
 /* mla_compress_kv: latent [seq][d_c] = kv [seq][d_h] . down [d_h][d_c]. */

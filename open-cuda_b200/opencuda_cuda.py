@@ -40,6 +40,7 @@ vp = C.c_void_p
 sz = C.c_size_t
 ci = C.c_int
 cf = C.c_float
+i64 = C.c_int64
 
 
 class OcError(RuntimeError):
@@ -93,6 +94,15 @@ _SIGS = {
     "oc_flash_attention_fwd": (ci, [vp, vp, vp, vp, ci, ci, ci, ci, cf, ci, vp]),
     "oc_sdpa_workspace_size": (ci, [ci, C.POINTER(sz)]),
     "oc_sdpa": (ci, [vp, vp, vp, vp, ci, ci, vp, sz, vp]),
+    "oc_kv_scratch_size": (ci, [ci, ci, C.POINTER(sz)]),
+    "oc_kv_extend": (ci, [vp, vp, vp, ci, vp]),
+    "oc_kv_fork": (ci, [vp, vp, vp, ci, vp]),
+    "oc_kv_free": (ci, [vp, vp, ci, vp]),
+    "oc_kv_compact": (ci, [vp, vp]),
+    "oc_kv_copy_pages": (ci, [vp, vp, vp, ci, vp]),
+    "oc_kv_append": (ci, [vp, ci, ci, ci, vp, vp, ci, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, cf, vp, ci, ci, vp]),
+    "oc_kv_attention_workspace_size": (ci, [vp, ci, ci, ci, C.POINTER(sz)]),
+    "oc_kv_attention": (ci, [vp, ci, ci, ci, vp, vp, ci, vp, i64, vp, i64, cf, ci, ci, vp, sz, vp]),
     "oc_mla_compress_kv": (ci, [ci, ci, ci, vp, vp, vp, vp]),
     "oc_mla_decompress_kv": (ci, [ci, ci, ci, vp, vp, vp, vp]),
     "oc_device_launch": (ci, [vp, C.c_char_p, vp, vp, sz]),

@@ -14,6 +14,14 @@ pub const OC_ERR_NO_DEVICE: c_int = 100;
 pub const OC_ERR_NOT_SUPPORTED: c_int = 801;
 pub const OC_ERR_TIMEOUT: c_int = 702;
 
+pub const OC_KV_F32: c_int = 0;
+pub const OC_KV_F16: c_int = 1;
+pub const OC_KV_BF16: c_int = 2;
+pub const OC_KV_NO_PAGES: c_int = 1;
+pub const OC_KV_BAD_SEQUENCE: c_int = 2;
+pub const OC_KV_ROW_FULL: c_int = 4;
+pub const OC_KV_BAD_PAGE: c_int = 8;
+
 pub const OC_ARG_PTR: c_int = 0;
 pub const OC_ARG_U32: c_int = 1;
 pub const OC_ARG_I32: c_int = 2;
@@ -38,6 +46,27 @@ pub struct oc_device_info {
     pub total_memory: u64,
     pub compute_units: u32,
     pub name: [c_char; 256],
+}
+
+/// The paged key/value cache: device addresses and shape.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct oc_kv_cache {
+    pub k: u64,
+    pub v: u64,
+    pub page_table: u64,
+    pub seq_len: u64,
+    pub refcount: u64,
+    pub status: u64,
+    pub scratch: u64,
+    pub dtype: c_int,
+    pub num_layers: c_int,
+    pub num_pages: c_int,
+    pub kv_heads: c_int,
+    pub page_size: c_int,
+    pub head_dim: c_int,
+    pub max_seqs: c_int,
+    pub max_pages_per_seq: c_int,
 }
 
 #[repr(C)]
@@ -263,5 +292,80 @@ extern "C" {
         out_tokens: *mut u32,
         out_logits: *mut f32,
         produced: *mut c_int,
+    ) -> c_int;
+
+    pub fn oc_kv_scratch_size(num_pages: c_int, max_seqs: c_int, bytes: *mut usize) -> c_int;
+    pub fn oc_kv_extend(
+        cache: *const oc_kv_cache,
+        seqs: u64,
+        counts: u64,
+        n: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn oc_kv_fork(
+        cache: *const oc_kv_cache,
+        parents: u64,
+        children: u64,
+        n: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn oc_kv_free(cache: *const oc_kv_cache, seqs: u64, n: c_int, stream: *mut c_void) -> c_int;
+    pub fn oc_kv_compact(cache: *const oc_kv_cache, stream: *mut c_void) -> c_int;
+    pub fn oc_kv_copy_pages(
+        cache: *const oc_kv_cache,
+        src: u64,
+        dst: u64,
+        n: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn oc_kv_append(
+        cache: *const oc_kv_cache,
+        layer: c_int,
+        tokens: c_int,
+        n: c_int,
+        cu: u64,
+        seqs: u64,
+        q_heads: c_int,
+        q: u64,
+        q_stride: i64,
+        k: u64,
+        k_stride: i64,
+        v: u64,
+        v_stride: i64,
+        q_out: u64,
+        q_out_stride: i64,
+        q_weight: u64,
+        k_weight: u64,
+        eps: f32,
+        inv_freq: u64,
+        rot_dim: c_int,
+        interleaved: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn oc_kv_attention_workspace_size(
+        cache: *const oc_kv_cache,
+        tokens: c_int,
+        n: c_int,
+        q_heads: c_int,
+        bytes: *mut usize,
+    ) -> c_int;
+    pub fn oc_kv_attention(
+        cache: *const oc_kv_cache,
+        layer: c_int,
+        tokens: c_int,
+        n: c_int,
+        cu: u64,
+        seqs: u64,
+        q_heads: c_int,
+        q: u64,
+        q_stride: i64,
+        out: u64,
+        out_stride: i64,
+        scale: f32,
+        causal: c_int,
+        window: c_int,
+        workspace: u64,
+        workspace_bytes: usize,
+        stream: *mut c_void,
     ) -> c_int;
 }
