@@ -3,7 +3,7 @@
 #include <map>
 
 #include "oc_kv_plan.cuh"
-#include "oc_kv_rows.cuh"
+#include "oc_kv_mma.cuh"
 
 namespace oc {
 
@@ -57,10 +57,14 @@ __global__ void __launch_bounds__(128) kv_merge_kernel(KvAttn a, int dp) {
   const float ls = lsum[0] + lsum[1] + lsum[2] + lsum[3];
   const int rr = cur.it.r0 + r, g = a.p.group;
   T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + rr / g) * a.os + (int64_t)(cur.h * g + rr % g) * d;
+  bool bad = false;
   for (int e = threadIdx.x; e < d; e += blockDim.x) {
-    const float o = part[0][e] + part[1][e] + part[2][e] + part[3][e];
-    out[e] = kv_from<T>(ls == 0.0f ? 0.0f : o / ls);
+    const float o = ls == 0.0f ? 0.0f : (part[0][e] + part[1][e] + part[2][e] + part[3][e]) / ls;
+    out[e] = kv_from<T>(o);
+    bad |= !isfinite(o);
   }
+  // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
+  if (__syncthreads_or(bad) && warp == 0) kv_row_exact<T>(a, cur.s, cur.h, rr);
 }
 
 // CTAs of a kernel that fit the GPU at once, remembered per device and kernel.
@@ -92,31 +96,51 @@ struct KvLaunch {
 };
 
 template <typename K>
-static KvLaunch rows_launch(int min_units) {
+static KvLaunch shape_of(void (*kern)(KvAttn), int min_units) {
   KvLaunch l;
-  l.kern = kv_rows_kernel<K>;
+  l.kern = kern;
   l.br = K::ROWS, l.bk = K::BK, l.dp = K::DP, l.threads = K::THREADS, l.min_units = min_units, l.smem = K::SMEM;
   return l;
 }
 
+// On the CUDA cores; `rows`: the most that a sequence's kv head can have.
 template <typename T>
 static KvLaunch scalar_launch(int d, int rows) {
+  auto go = [](auto k) { return shape_of<decltype(k)>(kv_rows_kernel<decltype(k)>, 4); };
   if constexpr (sizeof(T) == 4) {
-    if (d <= 64) return rows <= 1 ? rows_launch<KvRows<T, 64, 1>>(4) : rows_launch<KvRows<T, 64, 8>>(4);
-    if (d <= 128) return rows <= 1 ? rows_launch<KvRows<T, 128, 1>>(4) : rows_launch<KvRows<T, 128, 8>>(4);
-    return rows_launch<KvRows<T, 256, 4>>(4);
+    if (d <= 64) return rows <= 1 ? go(KvRows<T, 64, 1>()) : go(KvRows<T, 64, 8>());
+    if (d <= 128) return rows <= 1 ? go(KvRows<T, 128, 1>()) : go(KvRows<T, 128, 8>());
+    return go(KvRows<T, 256, 4>());
   } else {
-    if (d <= 64) return rows_launch<KvRows<T, 64, 8>>(4);
-    if (d <= 128) return rows_launch<KvRows<T, 128, 8>>(4);
-    return rows_launch<KvRows<T, 256, 4>>(4);
+    if (d <= 64) return go(KvRows<T, 64, 4>());
+    if (d <= 128) return go(KvRows<T, 128, 4>());
+    return go(KvRows<T, 256, 4>());
   }
 }
+
+// On warp-level matrix instructions.
+template <typename T>
+static KvLaunch mma_launch(int d, int rows) {
+  auto go = [](auto k) { return shape_of<decltype(k)>(kv_mma_kernel<decltype(k)>, 2); };
+  if (d <= 64) return rows <= 16 ? go(KvMma<T, 64, 1>()) : go(KvMma<T, 64, 2>());
+  if (d <= 96) return rows <= 16 ? go(KvMma<T, 96, 1>()) : go(KvMma<T, 96, 2>());
+  if (d <= 128) return rows <= 16 ? go(KvMma<T, 128, 1>()) : go(KvMma<T, 128, 2>());
+  return go(KvMma<T, 256, 1>());
+}
+
+// Rows of the pools are whole, aligned 16-byte chunks.
+static bool vector_rows(const KvView& c, size_t esize) { return c.d * esize % 16 == 0 && aligned16(c.k) && aligned16(c.v); }
 
 // The launches of a call, each over its class of sequences.
 template <typename T>
 static int pick(const KvView& c, int tokens, int n, int q_heads, KvLaunch (&out)[2]) {
   const int group = q_heads / c.hk;
-  out[0] = scalar_launch<T>(c.d, tokens <= n ? group : INT_MAX);
+  const int rows = tokens <= n ? group : INT_MAX;
+  if constexpr (sizeof(T) == 2) {
+    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, rows) : scalar_launch<T>(c.d, rows);
+  } else {
+    out[0] = scalar_launch<T>(c.d, rows);
+  }
   for (int i = 0; i < 1; ++i) out[i].ctas = resident_ctas(reinterpret_cast<const void*>(out[i].kern), out[i].threads, out[i].smem);
   return 1;
 }
@@ -195,8 +219,9 @@ int oc_kv_attention(const oc_kv_cache* cache, int layer, int tokens, int n, cons
   a.layer_off = (((size_t)layer * c.pages * c.hk) << c.ps_shift) * c.d;
   a.q = q, a.out = out, a.qs = q_stride, a.os = out_stride;
   a.scale2 = scale * 1.44269504088896341f;
-  a.vec = c.d * es % 16 == 0 && aligned16(c.k) && aligned16(c.v);
+  a.vec = vector_rows(c, es);
   a.qvec = c.d * es % 16 == 0 && aligned16(q) && q_stride * es % 16 == 0;
+  a.ovec = c.d % 2 == 0 && reinterpret_cast<uintptr_t>(out) % (2 * es) == 0 && out_stride % 2 == 0;
   a.ws = nullptr;
   a.dev_status = device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);

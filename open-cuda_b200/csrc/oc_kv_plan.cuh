@@ -160,6 +160,7 @@ struct KvAttn {
   float scale2;  // scale * log2(e)
   int vec;       // rows of the pools are whole 16-byte chunks
   int qvec;      // rows of q are
+  int ovec;      // pairs of elements of out are 4-byte aligned
   float* ws;
   int* dev_status;
 };
