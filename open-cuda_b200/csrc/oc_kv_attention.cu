@@ -7,30 +7,20 @@
 
 namespace oc {
 
-// Joins the pieces of one item that a cut went through: blockIdx.x = the cut
-// (before CTA blockIdx.x + 1), blockIdx.y = the row.  Only the first cut
-// inside an item does it.
+// Joins the pieces of one item that a cut went through: blockIdx.x = the CTA
+// whose run it began in, blockIdx.y = the row.
 template <typename T>
 __global__ void __launch_bounds__(128) kv_merge_kernel(KvAttn a, int dp) {
-  __shared__ KvPlanShared sh;
   __shared__ float part[4][256], lsum[4];
   const KvView& c = a.c;
-  KvCursor cur;
-  int64_t chunk;
-  const int cut = blockIdx.x + 1;
-  // the batch was complete before the kernel that this one follows began
-  const int64_t total = plan_locate(a.p, c, a.bt, cut, &sh, &chunk, cur);
   pdl_wait();
-  if (total == 0 || cur.at == 0) return;
-  const int64_t u = chunk * cut, begin = u - cur.at, end = begin + cur.it.units;
-  if (begin < u - chunk) return;  // an earlier cut's
-  const int r = blockIdx.y;
-  if (r >= cur.it.rows) return;
-  const int pieces = 2 + (int)((end - u - 1) / chunk);
+  const KvCut cut = reinterpret_cast<const KvCut*>(a.ws)[blockIdx.x];
+  const int r = blockIdx.y, pieces = cut.pieces;
+  if (pieces == 0 || r >= cut.rows) return;
   const size_t step = 2 * plan_slot_floats(a.p.br, dp);
-  // piece 0 is slot 1 of CTA cut - 1, piece i slot 0 of CTA cut - 1 + i
-  const float* first = plan_slot(a, cut - 1, 1, dp);
-  const float* rest = plan_slot(a, cut, 0, dp);
+  // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
+  const float* first = plan_slot(a, blockIdx.x, 1, dp);
+  const float* rest = plan_slot(a, blockIdx.x + 1, 0, dp);
   auto at = [&](int i) { return i == 0 ? first : rest + (size_t)(i - 1) * step; };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, br = a.p.br, d = c.d;
   float m = -INFINITY;
@@ -55,8 +45,8 @@ __global__ void __launch_bounds__(128) kv_merge_kernel(KvAttn a, int dp) {
   if (lane == 0) lsum[warp] = l;
   __syncthreads();
   const float ls = lsum[0] + lsum[1] + lsum[2] + lsum[3];
-  const int rr = cur.it.r0 + r, g = a.p.group;
-  T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + rr / g) * a.os + (int64_t)(cur.h * g + rr % g) * d;
+  const int rr = cut.r0 + r, g = a.p.group;
+  T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + rr / g) * a.os + (int64_t)(cut.h * g + rr % g) * d;
   bool bad = false;
   for (int e = threadIdx.x; e < d; e += blockDim.x) {
     const float o = ls == 0.0f ? 0.0f : (part[0][e] + part[1][e] + part[2][e] + part[3][e]) / ls;
@@ -64,7 +54,7 @@ __global__ void __launch_bounds__(128) kv_merge_kernel(KvAttn a, int dp) {
     bad |= !isfinite(o);
   }
   // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
-  if (__syncthreads_or(bad) && warp == 0) kv_row_exact<T>(a, cur.s, cur.h, rr);
+  if (__syncthreads_or(bad) && warp == 0) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
 }
 
 // CTAs of a kernel that fit the GPU at once, remembered per device and kernel.
@@ -93,6 +83,7 @@ struct KvLaunch {
   int rows_min = 0, rows_max = INT_MAX;
   size_t smem = 0;
   int ctas = 0;
+  int merge_rows = 0;  // rows that an item of a call can have
 };
 
 template <typename K>
@@ -141,13 +132,19 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, KvLaunch (&out)
   } else {
     out[0] = scalar_launch<T>(c.d, rows);
   }
-  for (int i = 0; i < 1; ++i) out[i].ctas = resident_ctas(reinterpret_cast<const void*>(out[i].kern), out[i].threads, out[i].smem);
-  return 1;
+  const int count = 1;
+  for (int i = 0; i < count; ++i) {
+    const void* fn = reinterpret_cast<const void*>(out[i].kern);
+    smem_attr_once(fn, out[i].smem);  // before the occupancy is asked for
+    out[i].ctas = resident_ctas(fn, out[i].threads, out[i].smem);
+    out[i].merge_rows = std::min(out[i].br, rows);
+  }
+  return count;
 }
 
 static size_t workspace_floats(const KvLaunch* l, int count) {
   size_t most = 0;
-  for (int i = 0; i < count; ++i) most = std::max(most, (size_t)l[i].ctas * 2 * plan_slot_floats(l[i].br, l[i].dp));
+  for (int i = 0; i < count; ++i) most = std::max(most, plan_cut_floats(l[i].ctas) + (size_t)l[i].ctas * 2 * plan_slot_floats(l[i].br, l[i].dp));
   return most;
 }
 
@@ -158,14 +155,14 @@ static int run(KvAttn a, int q_heads, void* ws, size_t ws_bytes, cudaStream_t s)
   OC_REQUIRE(ws && aligned16(ws) && ws_bytes >= workspace_floats(l, count) * sizeof(float),
              "kv_attention: workspace too small or not 16-byte aligned");
   for (int i = 0; i < count; ++i) {
-    a.p.br = l[i].br, a.p.bk = l[i].bk, a.p.rows_min = l[i].rows_min, a.p.rows_max = l[i].rows_max;
+    a.p.br = l[i].br, a.p.bk_shift = __builtin_ctz(l[i].bk), a.p.rows_min = l[i].rows_min, a.p.rows_max = l[i].rows_max;
     a.p.ctas = l[i].ctas, a.p.min_units = l[i].min_units;
     a.ws = static_cast<float*>(ws);
     if (!smem_attr_once(reinterpret_cast<const void*>(l[i].kern), l[i].smem))
       return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
     OC_CHECK_CUDA(launch_pdl_ex(l[i].kern, dim3(l[i].ctas), dim3(l[i].threads), l[i].smem, s, a));
     if (l[i].ctas > 1)
-      OC_CHECK_CUDA(launch_pdl_ex(kv_merge_kernel<T>, dim3(l[i].ctas - 1, l[i].br), dim3(128), 0, s, a, l[i].dp));
+      OC_CHECK_CUDA(launch_pdl_ex(kv_merge_kernel<T>, dim3(l[i].ctas - 1, l[i].merge_rows), dim3(128), 0, s, a, l[i].dp));
   }
   return OC_OK;
 }
@@ -214,6 +211,7 @@ int oc_kv_attention(const oc_kv_cache* cache, int layer, int tokens, int n, cons
   a.bt = KvBatch{cu, seqs, n, tokens};
   a.p = KvPlan{};
   a.p.group = q_heads / c.hk;
+  a.p.group_inv = a.p.group == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / a.p.group);
   a.p.causal = causal != 0;
   a.p.window = window;
   a.layer_off = (((size_t)layer * c.pages * c.hk) << c.ps_shift) * c.d;

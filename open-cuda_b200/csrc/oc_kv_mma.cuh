@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
   KvCursor cur;
   int64_t chunk;
   const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, cur);
+  if (threadIdx.x == 0) plan_no_cut(a);
   if (total == 0) return;
   int64_t left = min(chunk, total - chunk * blockIdx.x);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -177,20 +178,22 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
     auto offset = [&](int i) {
       return i < ntile ? kv_row_off(a, cur.s.s, cur.h, key0 + (lane & 15) + i * K::BK, it.lo, it.hi) : -1;
     };
-    int64_t next = offset(0);
+    int64_t ahead_off[NS];  // the page table is asked for the first tiles at once
+#pragma unroll
+    for (int s = 0; s < NS; ++s) ahead_off[s] = offset(s);
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
-      if (s < ntile) kv_load_tile<T, DP>(a, kb, vb, next, ring + s * K::STAGE, ring + s * K::STAGE + L::BYTES, lane);
+      if (s < ntile) kv_load_tile<T, DP>(a, kb, vb, ahead_off[s], ring + s * K::STAGE, ring + s * K::STAGE + L::BYTES, lane);
       cp_async_commit();
-      next = offset(s + 1);
     }
+    int64_t next = ahead_off[NS - 1];
     if (a.qvec) {
       for (int x = threadIdx.x; x < ROWS * (DP / 8); x += K::THREADS) {
         const int r = x / (DP / 8), e = x % (DP / 8) * 8, rr = it.r0 + r;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < it.rows && e < d)
-          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(cur.s.q0 + rr / g) * a.qs +
-                                              (int64_t)(cur.h * g + rr % g) * d + e);
+          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.qs +
+                                              (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e);
         *reinterpret_cast<uint4*>(sq + r * L::RB + e * 2) = v;
       }
     } else {
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
         const int r = x / DP, e = x % DP, rr = it.r0 + r;
         T v = kv_from<T>(0.0f);
         if (r < it.rows && e < d)
-          v = static_cast<const T*>(a.q)[(int64_t)(cur.s.q0 + rr / g) * a.qs + (int64_t)(cur.h * g + rr % g) * d + e];
+          v = static_cast<const T*>(a.q)[(int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.qs + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e];
         *reinterpret_cast<T*>(sq + r * L::RB + e * 2) = v;
       }
     }
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
           const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
           os.x *= inv, os.y *= inv;
           if (!isfinite(os.x) || !isfinite(os.y)) bad |= 1u << r;
-          T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + rr / g) * a.os + (int64_t)(cur.h * g + rr % g) * d + e;
+          T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.os + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e;
           if (a.ovec) {
             *reinterpret_cast<uint32_t*>(out) = kv_pack2<T>(os.x, os.y);
           } else {
@@ -396,6 +399,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
         if ((todo >> r) & 1u) kv_row_exact<T>(a, cur.s, cur.h, it.r0 + r);
       __syncthreads();
     }
+    if (t0 == 0 && !whole && threadIdx.x == 0) plan_cut(a, cur, it.units - t1, chunk);
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }

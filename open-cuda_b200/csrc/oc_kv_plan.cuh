@@ -21,17 +21,25 @@
 namespace oc {
 
 struct KvPlan {
-  int br, bk;              // query rows of an item, keys of a tile
+  int br, bk_shift;        // query rows of an item; log2 of the keys of a tile
   int rows_min, rows_max;  // sequences with rows_min < rows <= rows_max are this launch's
   int ctas, min_units;     // grid, and the shortest run worth a CTA of its own
   int group;               // G
+  uint32_t group_inv;      // floor(2^32 / G), 2^32 - 1 for 1
   int causal, window;
 };
+
+// r / G for 0 <= r < 2^31: the product with the inverse is at most one short.
+__device__ __forceinline__ int plan_token(const KvPlan& p, int r) {
+  int q = (int)__umulhi((uint32_t)r, p.group_inv);
+  if (r - q * p.group >= p.group) ++q;
+  return q;
+}
 
 // Keys [lo, hi) that rows [r0, r1] of a sequence see at all.
 __device__ __forceinline__ void plan_range(const KvPlan& p, const KvSeq& s, int r0, int r1, int& lo, int& hi) {
   const int before = s.len - s.nq;
-  const int first = before + r0 / p.group, last = before + r1 / p.group;
+  const int first = before + plan_token(p, r0), last = before + plan_token(p, r1);
   hi = p.causal ? min(s.len, max(last + 1, 0)) : s.len;
   lo = p.window > 0 ? (int)max((int64_t)0, (int64_t)first - p.window + 1) : 0;
   lo = min(lo, hi);
@@ -51,94 +59,142 @@ __device__ __forceinline__ KvItem plan_item(const KvPlan& p, const KvSeq& s, int
   it.r0 = j * p.br;
   it.rows = min(p.br, s.nq * p.group - it.r0);
   plan_range(p, s, it.r0, it.r0 + it.rows - 1, it.lo, it.hi);
-  it.tile0 = it.lo / p.bk;
-  it.units = max(1, (int)(((int64_t)it.hi + p.bk - 1) / p.bk) - it.tile0);
+  it.tile0 = it.lo >> p.bk_shift;
+  it.units = max(1, (int)(((int64_t)it.hi + (1 << p.bk_shift) - 1) >> p.bk_shift) - it.tile0);
   return it;
 }
 __device__ __forceinline__ int plan_blocks(const KvPlan& p, const KvSeq& s) {
   const int rows = s.nq * p.group;
   return rows > p.rows_min && rows <= p.rows_max ? (rows + p.br - 1) / p.br : 0;
 }
-// Units of one kv head of a sequence.
-__device__ __forceinline__ int64_t plan_head_units(const KvPlan& p, const KvSeq& s) {
-  int64_t u = 0;
-  const int nb = plan_blocks(p, s);
-  for (int j = 0; j < nb; ++j) u += plan_item(p, s, j).units;
-  return u;
-}
 
 // A place in the list of units.
 struct KvCursor {
   int b;            // entry of the batch
   KvSeq s;
-  int64_t head;     // units of one of its kv heads
+  int blocks;       // row blocks of the sequence
   int h, j;         // kv head, row block
   KvItem it;
   int at;           // unit within the item
 };
 
+constexpr int kPlanSmall = 8;  // row blocks that one thread sums by itself
+
 struct KvPlanShared {
   int64_t sums[33];
-  int64_t off;
-  int b;
+  int64_t off, head;
+  int b, j, at, big;
 };
+
+// Units of one kv head of a sequence, by all threads of the block.
+__device__ __forceinline__ int64_t plan_head_block(const KvPlan& p, const KvSeq& s, int blocks, KvPlanShared* sh) {
+  int64_t u = 0, total;
+  for (int j = threadIdx.x; j < blocks; j += blockDim.x) u += plan_item(p, s, j).units;
+  block_exclusive<int64_t>(u, sh->sums, &total);
+  return total;
+}
 
 // Sets the cursor to unit index * chunk.  Returns the number of units that
 // exist (0: none at or after that place); *chunk is the length of a run.
 // Block-wide: all threads call it with the same arguments and leave with the
-// same cursor.
+// same cursor.  A thread sums the sequences that are its own; sequences of
+// many row blocks (a chunk of 2048 tokens has hundreds) are summed by all.
 __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c, const KvBatch& bt, int index,
                                                KvPlanShared* sh, int64_t* chunk, KvCursor& cur) {
-  const int per = (bt.n + blockDim.x - 1) / blockDim.x;
-  const int b0 = min(bt.n, (int)threadIdx.x * per), b1 = min(bt.n, b0 + per);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += plan_head_units(p, kv_seq(c, bt, b)) * c.hk;
-  int64_t total;
-  int64_t before = block_exclusive<int64_t>(mine, sh->sums, &total);
-  const int64_t run = max((int64_t)p.min_units, (total + p.ctas - 1) / p.ctas);
-  *chunk = run;
-  const int64_t u = run * index;
-  if (u >= total) return 0;
-  if (before <= u && u < before + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const int64_t w = plan_head_units(p, kv_seq(c, bt, b)) * c.hk;
-      if (u < before + w) {
-        sh->b = b;
-        sh->off = u - before;
-        break;
-      }
-      before += w;
+  int64_t total = 0, u;
+  bool have = false;
+  if (threadIdx.x == 0) sh->b = -1;
+  // the units of the sequences, blockDim at a time: the sum first, then (a
+  // second round) the place; one round does both when it sees all sequences
+  const bool once = bt.n <= (int)blockDim.x;
+  for (int round = once ? 1 : 0; round < 2; ++round) {
+    if (round == 1 && !once) {
+      *chunk = max((int64_t)p.min_units, (total + p.ctas - 1) / p.ctas);
+      u = *chunk * index;
+      if (u >= total) return 0;
+      have = true;
     }
+    int64_t done = 0;
+    for (int b0 = 0; b0 < bt.n; b0 += blockDim.x) {
+      const int b = b0 + threadIdx.x;
+      KvSeq s{-1, 0, 0, 0};
+      if (b < bt.n) s = kv_seq(c, bt, b);
+      const int blocks = plan_blocks(p, s);
+      int64_t head = 0;
+      if (blocks <= kPlanSmall)
+        for (int j = 0; j < blocks; ++j) head += plan_item(p, s, j).units;
+      if (__syncthreads_or(blocks > kPlanSmall)) {
+        // one after another, in order: the next one is the lowest left
+        int left = blocks > kPlanSmall;
+        for (;;) {
+          if (threadIdx.x == 0) sh->big = INT_MAX;
+          __syncthreads();
+          if (left) atomicMin(&sh->big, b);
+          __syncthreads();
+          const int big = sh->big;
+          if (big == INT_MAX) break;
+          const KvSeq t = kv_seq(c, bt, big);
+          const int64_t sum = plan_head_block(p, t, plan_blocks(p, t), sh);
+          if (b == big) head = sum, left = 0;
+        }
+      }
+      int64_t sum;
+      const int64_t before = done + block_exclusive<int64_t>(head * c.hk, sh->sums, &sum);
+      done += sum;
+      if (once) {
+        *chunk = max((int64_t)p.min_units, (done + p.ctas - 1) / p.ctas);
+        u = *chunk * index;
+        if (u >= done) return 0;
+        have = true;
+      }
+      if (have && before <= u && u < before + head * c.hk) sh->b = b, sh->off = u - before, sh->head = head;
+      __syncthreads();
+      if (have && sh->b >= 0) break;
+    }
+    total = once || round == 0 ? done : total;
   }
-  __syncthreads();
   cur.b = sh->b;
   cur.s = kv_seq(c, bt, cur.b);
-  cur.head = plan_head_units(p, cur.s);
+  cur.blocks = plan_blocks(p, cur.s);
   int64_t off = sh->off;
-  cur.h = (int)(off / cur.head);
-  off -= cur.h * cur.head;
-  cur.j = 0;
-  for (;;) {
-    cur.it = plan_item(p, cur.s, cur.j);
-    if (off < cur.it.units) break;
-    off -= cur.it.units;
-    ++cur.j;
+  if (cur.blocks == 1) {
+    cur.h = (int)(off / sh->head);
+    cur.j = 0;
+    cur.it = plan_item(p, cur.s, 0);
+    cur.at = (int)(off - cur.h * sh->head);
+    return total;
   }
-  cur.at = (int)off;
+  cur.h = (int)(off / sh->head);
+  off -= cur.h * sh->head;
+  int64_t before = 0;
+  for (int j0 = 0;; j0 += blockDim.x) {
+    const int j = j0 + threadIdx.x;
+    const int64_t w = j < cur.blocks ? plan_item(p, cur.s, j).units : 0;
+    int64_t sum;
+    const int64_t mine = before + block_exclusive<int64_t>(w, sh->sums, &sum);
+    if (mine <= off && off < mine + w) sh->j = j, sh->at = (int)(off - mine);
+    before += sum;
+    if (off < before || j0 + (int)blockDim.x >= cur.blocks) break;
+  }
+  __syncthreads();
+  cur.j = sh->j;
+  cur.at = sh->at;
+  cur.it = plan_item(p, cur.s, cur.j);
   return total;
 }
 
 // The next item's first unit; false at the end of the list.
 __device__ __forceinline__ bool plan_next(const KvPlan& p, const KvView& c, const KvBatch& bt, KvCursor& cur) {
   cur.at = 0;
-  if (++cur.j >= plan_blocks(p, cur.s)) {
+  if (++cur.j >= cur.blocks) {
     cur.j = 0;
     if (++cur.h >= c.hk) {
       cur.h = 0;
       for (;;) {
         if (++cur.b >= bt.n) return false;
         cur.s = kv_seq(c, bt, cur.b);
-        if (plan_blocks(p, cur.s) > 0) break;
+        cur.blocks = plan_blocks(p, cur.s);
+        if (cur.blocks > 0) break;
       }
     }
   }
@@ -146,8 +202,16 @@ __device__ __forceinline__ bool plan_next(const KvPlan& p, const KvView& c, cons
   return true;
 }
 
-// Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp], f32.
+// What the cut behind a CTA's run goes through, for the merge kernel.
+struct KvCut {
+  int pieces;  // 0: nothing
+  int b, h, r0, rows, q0, unused0, unused1;
+};
+
+// Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp], f32;
+// in front of them the cuts, one per CTA.
 __host__ __device__ inline size_t plan_slot_floats(int br, int dp) { return (size_t)br * (dp + 2); }
+__host__ __device__ inline size_t plan_cut_floats(int ctas) { return (size_t)ctas * (sizeof(KvCut) / sizeof(float)); }
 
 struct KvAttn {
   KvView c;
@@ -166,7 +230,17 @@ struct KvAttn {
 };
 
 __device__ __forceinline__ float* plan_slot(const KvAttn& a, int cta, int slot, int dp) {
-  return a.ws + ((size_t)cta * 2 + slot) * plan_slot_floats(a.p.br, dp);
+  return a.ws + plan_cut_floats(a.p.ctas) + ((size_t)cta * 2 + slot) * plan_slot_floats(a.p.br, dp);
+}
+
+// One thread of a CTA: what its run leaves to the CTAs behind it.
+__device__ __forceinline__ void plan_no_cut(const KvAttn& a) {
+  reinterpret_cast<KvCut*>(a.ws)[blockIdx.x].pieces = 0;
+}
+// The last item of its run began there and goes on: rest = its units behind the run.
+__device__ __forceinline__ void plan_cut(const KvAttn& a, const KvCursor& cur, int rest, int64_t chunk) {
+  reinterpret_cast<KvCut*>(a.ws)[blockIdx.x] =
+      KvCut{2 + (int)((rest - 1) / chunk), cur.b, cur.h, cur.it.r0, cur.it.rows, cur.s.q0, 0, 0};
 }
 
 }  // namespace oc

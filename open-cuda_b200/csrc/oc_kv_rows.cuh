@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
   KvCursor cur;
   int64_t chunk;
   const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, cur);
+  if (threadIdx.x == 0) plan_no_cut(a);
   if (total == 0) return;
   const int64_t u0 = chunk * blockIdx.x;
   int64_t left = min(chunk, total - u0);
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
       const bool live = r < it.rows;
       const int rr = it.r0 + r;
       if (live) plan_row_range(a.p, cur.s, rr, lo[r], hi[r]);
-      const T* src = static_cast<const T*>(a.q) + (int64_t)(cur.s.q0 + rr / g) * a.qs + (int64_t)(cur.h * g + rr % g) * d;
+      const T* src = static_cast<const T*>(a.q) + (int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.qs + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d;
 #pragma unroll
       for (int i = 0; i < F; ++i) {
         const int e = (l16 + 16 * (i / VN)) * VN + i % VN;
@@ -165,13 +166,15 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
     const int ntile = t1 - t0;
     const int key0 = (it.tile0 + t0) * K::BK + warp * 16 + l16;
     auto offset = [&](int i) { return i < ntile ? kv_row_off(a, cur.s.s, cur.h, key0 + i * K::BK, it.lo, it.hi) : -1; };
-    int64_t next = offset(0);
+    int64_t ahead_off[NS];  // the page table is asked for the first tiles at once
+#pragma unroll
+    for (int s = 0; s < NS; ++s) ahead_off[s] = offset(s);
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
-      if (s < ntile) kv_load_tile<T, DP>(a, kb, vb, next, ring + s * K::STAGE, ring + s * K::STAGE + L::BYTES, lane);
+      if (s < ntile) kv_load_tile<T, DP>(a, kb, vb, ahead_off[s], ring + s * K::STAGE, ring + s * K::STAGE + L::BYTES, lane);
       cp_async_commit();
-      next = offset(s + 1);
     }
+    int64_t next = ahead_off[NS - 1];
     for (int i = 0; i < ntile; ++i) {
       cp_async_wait<NS - 2>();
       __syncwarp();
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
       if (whole) {
         const int rr = it.r0 + r;
         if (e < d)
-          static_cast<T*>(a.out)[(int64_t)(cur.s.q0 + rr / g) * a.os + (int64_t)(cur.h * g + rr % g) * d + e] =
+          static_cast<T*>(a.out)[(int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.os + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e] =
               kv_from<T>(ls == 0.0f ? 0.0f : os / ls);
       } else {
         if (e == 0) slot[r] = mm, slot[ROWS + r] = ls;
@@ -298,6 +301,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
       }
     }
     __syncthreads();
+    if (t0 == 0 && !whole && threadIdx.x == 0) plan_cut(a, cur, it.units - t1, chunk);
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }

@@ -75,13 +75,15 @@ class KVCache:
         self._c = _Cache(k.data_ptr(), v.data_ptr(), page_table.data_ptr(), seq_len.data_ptr(), refcount.data_ptr(), status.data_ptr(),
                          self.scratch.data_ptr(), dtypes[k.dtype], layers, pages, heads, page_size, dim, *page_table.shape)
         self._p = C.byref(self._c)
-        self._index = k.device.index
-        self._int32 = torch.int32
-        self._cuda = torch.cuda
-        self._empty = torch.empty
-        self._ws_bytes = {}
+        # what every call needs: one attribute away
+        lib = oc.lib()
+        self._torch, self._index, self._int32, self._f32 = torch, k.device.index, torch.int32, torch.float32
+        self._current_device, self._raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        self._append, self._attention, self._extend, self._fork = lib.oc_kv_append, lib.oc_kv_attention, lib.oc_kv_extend, lib.oc_kv_fork
+        self._free, self._compact, self._copy = lib.oc_kv_free, lib.oc_kv_compact, lib.oc_kv_copy_pages
+        self._ws_bytes, self._workspaces = {}, {}
         ws = oc.sz(0)
-        oc.check(oc.lib().oc_kv_attention_workspace_size(self._p, 0, 0, heads, C.byref(ws)))  # checks the shape as a whole
+        oc.check(lib.oc_kv_attention_workspace_size(self._p, 0, 0, heads, C.byref(ws)))  # checks the shape as a whole
 
     @classmethod
     def create(cls, layers, pages, page_size, kv_heads, head_dim, dtype, max_seqs, max_pages_per_seq, device="cuda"):
@@ -100,34 +102,56 @@ class KVCache:
         return t.numel()
 
     def _batch(self, tokens, cu, seqs):
+        """Entries of the batch, and the addresses of cu and seqs."""
         if cu is None:
-            n = tokens
+            n, cp = tokens, None
         else:
-            n = self._ids(cu, "cu") - 1
+            n, cp = self._ids(cu, "cu") - 1, cu.data_ptr()
             if n < 0:
                 raise ValueError("kv_cache: cu holds one number more than there are sequences")
-        if seqs is not None and self._ids(seqs, "seqs") != n:
+        if seqs is None:
+            return n, cp, None
+        if self._ids(seqs, "seqs") != n:
             raise ValueError(f"kv_cache: {seqs.numel()} sequences for {n} entries")
-        return n
+        return n, cp, seqs.data_ptr()
 
-    def _rows(self, t, heads, what):
+    def _rows(self, t, tokens, heads, what):
         """Token stride of a [tokens, heads, head_dim] tensor whose tokens are contiguous."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"kv_cache: {what} is [tokens, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(t.shape)}")
+        shape, d = t.shape, self.head_dim
+        if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or shape[2] != d:
+            raise ValueError(f"kv_cache: {what} is [{tokens}, {heads}, {d}], got {tuple(shape)}")
         if t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"kv_cache: {what} is {self.dtype} on {self.device}")
-        st = t.stride()
-        if (t.shape[2] > 1 and st[2] != 1) or (t.shape[1] > 1 and st[1] != self.head_dim):
+        s0, s1, s2 = t.stride()
+        if (s2 != 1 and d > 1) or (s1 != d and heads > 1):
             raise ValueError(f"kv_cache: the heads of a token of {what} must be contiguous")
-        return max(st[0], t.shape[1] * self.head_dim) if t.shape[0] <= 1 else st[0]
+        return s0 if tokens > 1 else max(s0, heads * d)
 
     def _call(self, fn, *args):
         """Calls fn on the cache's device and that device's current stream."""
-        if self._cuda.current_device() == self._index:
-            oc.check(fn(self._p, *args, self._cuda.current_stream().cuda_stream))
+        index = self._index
+        if self._current_device() == index:
+            rc = fn(self._p, *args, self._raw_stream(index))
         else:
-            with self._cuda.device(self._index):
-                oc.check(fn(self._p, *args, self._cuda.current_stream().cuda_stream))
+            with self._torch.cuda.device(index):
+                rc = fn(self._p, *args, self._raw_stream(index))
+        if rc:
+            oc.check(rc)
+
+    def _workspace(self, need):
+        """Scratch of one attention call: eager calls of one stream run one
+        after another and share a buffer; a captured call gets its own, which
+        its graph keeps."""
+        stream = self._raw_stream(self._index)
+        if self._torch.cuda.is_current_stream_capturing():
+            return self._new_bytes(need)
+        ws = self._workspaces.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self._workspaces[stream] = self._new_bytes(need)
+        return ws
+
+    def _new_bytes(self, need):
+        return self._torch.empty(need, dtype=self._torch.uint8, device=self.device)
 
     # -- bookkeeping --
 
@@ -137,7 +161,7 @@ class KVCache:
         n = self._ids(seqs, "seqs")
         if self._ids(counts, "counts") != n:
             raise ValueError("kv_cache: one count per sequence")
-        self._call(oc.lib().oc_kv_extend, seqs.data_ptr(), counts.data_ptr(), n)
+        self._call(self._extend, seqs.data_ptr(), counts.data_ptr(), n)
 
     def fork(self, parents, children):
         """children[i] (empty) becomes a copy of parents[i]: full pages are
@@ -145,23 +169,23 @@ class KVCache:
         n = self._ids(parents, "parents")
         if self._ids(children, "children") != n:
             raise ValueError("kv_cache: one parent per child")
-        self._call(oc.lib().oc_kv_fork, parents.data_ptr(), children.data_ptr(), n)
+        self._call(self._fork, parents.data_ptr(), children.data_ptr(), n)
 
     def free(self, seqs):
         """The sequences give their pages back."""
         n = self._ids(seqs, "seqs")
-        self._call(oc.lib().oc_kv_free, seqs.data_ptr(), n)
+        self._call(self._free, seqs.data_ptr(), n)
 
     def compact(self):
         """Moves the pages in use to the pool's front."""
-        self._call(oc.lib().oc_kv_compact)
+        self._call(self._compact)
 
     def copy_pages(self, src, dst):
         """Page dst[i] := page src[i] over all layers; tables and counts stay."""
         n = self._ids(src, "src")
         if self._ids(dst, "dst") != n:
             raise ValueError("kv_cache: one destination per source")
-        self._call(oc.lib().oc_kv_copy_pages, src.data_ptr(), dst.data_ptr(), n)
+        self._call(self._copy, src.data_ptr(), dst.data_ptr(), n)
 
     def check(self):
         """Waits for the cache's device and raises ValueError if a call since
@@ -180,62 +204,65 @@ class KVCache:
         head_dim] and keys [tokens, kv_heads, head_dim], keys and values
         written to their pages.  Returns the queries (q_out, or a new tensor;
         q None: keys and values alone)."""
-        ks, vs = self._rows(k, self.kv_heads, "k"), self._rows(v, self.kv_heads, "v")
-        tokens = k.shape[0]
-        n = self._batch(tokens, cu, seqs)
-        heads = qs = os_ = qp = op = 0
+        tokens, d = k.shape[0], self.head_dim
+        ks, vs = self._rows(k, tokens, self.kv_heads, "k"), self._rows(v, tokens, self.kv_heads, "v")
+        n, cp, sp = self._batch(tokens, cu, seqs)
+        heads = qs = os_ = 0
+        qp = op = None
         if q is not None:
-            qs, heads = self._rows(q, None, "q"), q.shape[1]
+            heads = q.shape[1]
+            qs = self._rows(q, tokens, heads, "q")
             if q_out is None:
-                q_out = self._empty(q.shape, dtype=self.dtype, device=self.device)
-            os_ = self._rows(q_out, heads, "q_out")
-            if q.shape[0] != tokens or q_out.shape[0] != tokens:
-                raise ValueError("kv_cache: q, k, v and q_out have the same tokens")
+                q_out = q.new_empty(q.shape)
+                os_ = heads * d
+            else:
+                os_ = self._rows(q_out, tokens, heads, "q_out")
             qp, op = q.data_ptr(), q_out.data_ptr()
-        if v.shape[0] != tokens:
-            raise ValueError("kv_cache: q, k, v and q_out have the same tokens")
-        wp = []
-        for w in (q_weight, k_weight):
-            if w is not None and (w.shape != (self.head_dim,) or w.dtype != self.dtype or not w.is_contiguous() or w.device != self.device):
-                raise ValueError(f"kv_cache: a norm's weight is [{self.head_dim}] {self.dtype} on {self.device}")
-            wp.append(None if w is None else w.data_ptr())
-        rot, ip = 0, None
+        qw = kw = ip = None
+        rot = 0
+        if q_weight is not None:
+            qw = self._weight(q_weight)
+        if k_weight is not None:
+            kw = self._weight(k_weight)
         if inv_freq is not None:
-            if inv_freq.dim() != 1 or str(inv_freq.dtype) != "torch.float32" or not inv_freq.is_contiguous() or inv_freq.device != self.device:
+            if inv_freq.dim() != 1 or inv_freq.dtype != self._f32 or not inv_freq.is_contiguous() or inv_freq.device != self.device:
                 raise ValueError(f"kv_cache: inv_freq is a float32 vector on {self.device}")
             rot, ip = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-        self._call(oc.lib().oc_kv_append, layer, tokens, n, None if cu is None else cu.data_ptr(), None if seqs is None else seqs.data_ptr(),
-                   heads, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, op, os_, wp[0], wp[1], eps, ip, rot, int(interleaved))
+        self._call(self._append, layer, tokens, n, cp, sp, heads, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, op, os_, qw, kw, eps, ip, rot,
+                   1 if interleaved else 0)
         return q_out
+
+    def _weight(self, w):
+        if w.shape != (self.head_dim,) or w.dtype != self.dtype or not w.is_contiguous() or w.device != self.device:
+            raise ValueError(f"kv_cache: a norm's weight is [{self.head_dim}] {self.dtype} on {self.device}")
+        return w.data_ptr()
 
     def attention(self, layer, q, cu=None, seqs=None, scale=None, causal=True, window=0, out=None):
         """softmax(scale q . K^T) V of the new tokens' queries [tokens,
         q_heads, head_dim] over their sequences' pages (scale None: 1 /
         sqrt(head_dim)); causal, and the last `window` keys alone when window
         > 0.  Rows of `out` behind the last sequence stay as they are."""
-        qs = self._rows(q, None, "q")
+        if q.dim() != 3:
+            raise ValueError(f"kv_cache: q is [tokens, q_heads, {self.head_dim}], got {tuple(q.shape)}")
         tokens, heads, d = q.shape
-        n = self._batch(tokens, cu, seqs)
+        qs = self._rows(q, tokens, heads, "q")
+        n, cp, sp = self._batch(tokens, cu, seqs)
         if out is None:
-            out = self._empty(q.shape, dtype=self.dtype, device=self.device)
-        elif out.shape[0] != tokens:
-            raise ValueError("kv_cache: out has q's shape")
-        os_ = self._rows(out, heads, "out")
-        key = (tokens, n, heads)
-        need = self._ws_bytes.get(key)
-        if need is None:
-            size = oc.sz(0)
-            with self._cuda.device(self._index):
-                oc.check(oc.lib().oc_kv_attention_workspace_size(self._p, tokens, n, heads, C.byref(size)))
-            if len(self._ws_bytes) > 4096:
-                self._ws_bytes.clear()
-            need = self._ws_bytes[key] = max(16, size.value)
-        ws = self._empty(need, dtype=self._torch_uint8, device=self.device)
-        self._call(oc.lib().oc_kv_attention, layer, tokens, n, None if cu is None else cu.data_ptr(), None if seqs is None else seqs.data_ptr(),
-                   heads, q.data_ptr(), qs, out.data_ptr(), os_, 1.0 / math.sqrt(d) if scale is None else scale, int(bool(causal)), window,
-                   ws.data_ptr(), need)
+            out = q.new_empty(q.shape)
+            os_ = heads * d
+        else:
+            os_ = self._rows(out, tokens, heads, "out")
+        need = self._ws_bytes.get((tokens, n, heads)) or self._workspace_size(tokens, n, heads)
+        ws = self._workspace(need)
+        self._call(self._attention, layer, tokens, n, cp, sp, heads, q.data_ptr(), qs, out.data_ptr(), os_,
+                   1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, window, ws.data_ptr(), need)
         return out
 
-    @property
-    def _torch_uint8(self):
-        return oc._torch().uint8
+    def _workspace_size(self, tokens, n, heads):
+        size = oc.sz(0)
+        with self._torch.cuda.device(self._index):
+            oc.check(oc.lib().oc_kv_attention_workspace_size(self._p, tokens, n, heads, C.byref(size)))
+        if len(self._ws_bytes) > 4096:
+            self._ws_bytes.clear()
+        self._ws_bytes[tokens, n, heads] = need = max(16, size.value)
+        return need
