@@ -3,58 +3,141 @@
 #include <map>
 
 #include "oc_kv_plan.cuh"
-#include "oc_kv_mma.cuh"
+#include "oc_kv_tile.cuh"
 
 namespace oc {
 
-// Joins the pieces of one item that a cut went through: blockIdx.x = the CTA
-// whose run it began in, blockIdx.y = the row.
-template <typename T>
-__global__ void __launch_bounds__(128) kv_merge_kernel(KvAttn a, int dp) {
-  __shared__ float part[4][256], lsum[4];
+constexpr int kMostCtas = 2048;  // of an attention kernel's grid
+
+// Joins the pieces of the items that cuts went through.  R rows of an item at
+// a time: one, its pieces shared by the 8 warps, for decode steps, where an
+// item of a long sequence has few rows and dozens of pieces; eight, a warp
+// each, for chunks, whose items have many rows and two or three pieces.  The
+// outputs are requested together with the maxima they are weighted by, so a
+// row costs one trip to memory.  Every CTA lists the cuts that went through
+// an item and takes its share of their rows: a CTA per possible cut and row
+// would mostly be launched to find nothing (2065 CTAs, 8 us, at 296 x 7).
+template <typename T, int R>
+__global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, int dp, int groups) {
+  constexpr int WARPS = 8, SPLIT = WARPS / R;  // warps that share a row
+  __shared__ float part[R == 1 ? WARPS : 1][256], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
+  __shared__ unsigned short list[kMostCtas];
+  __shared__ int wcount[WARPS];
   const KvView& c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, br = a.p.br, d = c.d;
   pdl_wait();
-  const KvCut cut = reinterpret_cast<const KvCut*>(a.ws)[blockIdx.x];
-  const int r = blockIdx.y, pieces = cut.pieces;
-  if (pieces == 0 || r >= cut.rows) return;
-  const size_t step = 2 * plan_slot_floats(a.p.br, dp);
-  // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
-  const float* first = plan_slot(a, blockIdx.x, 1, dp);
-  const float* rest = plan_slot(a, blockIdx.x + 1, 0, dp);
-  auto at = [&](int i) { return i == 0 ? first : rest + (size_t)(i - 1) * step; };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, br = a.p.br, d = c.d;
-  float m = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, at(i)[r]);
+  const KvCut* cuts = reinterpret_cast<const KvCut*>(a.ws);
+  int found = 0;
+  for (int i0 = 0; i0 < a.p.ctas; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const bool there = i < a.p.ctas && cuts[i].pieces > 0;
+    const uint32_t votes = __ballot_sync(0xffffffffu, there);
+    if (lane == 0) wcount[warp] = __popc(votes);
+    __syncthreads();
+    int at = found;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float base = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  float acc[8] = {};
-#pragma unroll 4
-  for (int i = warp; i < pieces; i += 4) {
-    const float* s = at(i);
-    const float w = exp2f(s[r] - base);
-    l = fmaf(w, s[br + r], l);
-    const float* o = s + 2 * br + (size_t)r * dp;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < d) acc[e] = fmaf(w, o[lane + 32 * e], acc[e]);
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) at += wcount[w];
+      found += wcount[w];
+    }
+    if (there) list[at + __popc(votes & ((1u << lane) - 1))] = (unsigned short)i;
+    __syncthreads();
   }
+  for (int task = blockIdx.x; task < found * groups; task += gridDim.x) {
+  const int cta = list[task / groups];
+  const KvCut cut = cuts[cta];
+  const int pieces = cut.pieces, r = (task % groups) * R + warp / SPLIT;
+  if (r >= cut.rows) continue;  // R == 1: the whole CTA; else the warp has nobody to meet
+  const size_t step = 2 * plan_slot_floats(br, dp);
+  // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
+  const float* first = plan_slot(a, cta, 1, dp);
+  const float* rest = plan_slot(a, cta + 1, 0, dp);
+  constexpr int U = 4;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc[2] = {};  // features 4 lane .. and 128 + 4 lane ..
+  for (int i0 = warp % SPLIT; i0 < pieces; i0 += SPLIT * U) {
+    float pm[U], pl[U];
+    float4 po[U][2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[warp][lane + 32 * e] = acc[e];
-  if (lane == 0) lsum[warp] = l;
-  __syncthreads();
-  const float ls = lsum[0] + lsum[1] + lsum[2] + lsum[3];
-  const int rr = cut.r0 + r, g = a.p.group;
-  T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + rr / g) * a.os + (int64_t)(cut.h * g + rr % g) * d;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * SPLIT;
+      pm[u] = -INFINITY, pl[u] = 0.0f;
+      po[u][0] = po[u][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i < pieces) {
+        const float* s = i == 0 ? first : rest + (size_t)(i - 1) * step;
+        const float* o = s + plan_slot_o(br) + (size_t)r * dp;
+        pm[u] = s[r];
+        pl[u] = s[br + r];
+        if (4 * lane < dp) po[u][0] = *reinterpret_cast<const float4*>(o + 4 * lane);
+        if (128 + 4 * lane < dp) po[u][1] = *reinterpret_cast<const float4*>(o + 128 + 4 * lane);
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+    const float base = mn == -INFINITY ? 0.0f : mn, corr = exp2f(m - base);
+    m = mn;
+    l *= corr;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) acc[k].x *= corr, acc[k].y *= corr, acc[k].z *= corr, acc[k].w *= corr;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = exp2f(pm[u] - base);
+      l = fmaf(w, pl[u], l);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        acc[k].x = fmaf(w, po[u][k].x, acc[k].x);
+        acc[k].y = fmaf(w, po[u][k].y, acc[k].y);
+        acc[k].z = fmaf(w, po[u][k].z, acc[k].z);
+        acc[k].w = fmaf(w, po[u][k].w, acc[k].w);
+      }
+    }
+  }
+  const int rr = cut.r0 + r, token = plan_token(a.p, rr);
+  T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + token) * a.os + (int64_t)(cut.h * a.p.group + rr - token * a.p.group) * d;
   bool bad = false;
-  for (int e = threadIdx.x; e < d; e += blockDim.x) {
-    const float o = ls == 0.0f ? 0.0f : (part[0][e] + part[1][e] + part[2][e] + part[3][e]) / ls;
-    out[e] = kv_from<T>(o);
-    bad |= !isfinite(o);
+  if constexpr (R == 1) {
+    *reinterpret_cast<float4*>(&part[warp][4 * lane]) = acc[0];
+    *reinterpret_cast<float4*>(&part[warp][128 + 4 * lane]) = acc[1];
+    if (lane == 0) ms[warp] = m, ls[warp] = l;
+    __syncthreads();
+    float mm = ms[0];
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) mm = fmaxf(mm, ms[k]);
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float sum = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float w = exp2f(ms[k] - base);
+      sum = fmaf(w, ls[k], sum);
+      o = fmaf(w, part[k][threadIdx.x], o);
+    }
+    if ((int)threadIdx.x < d) {
+      o = sum == 0.0f ? 0.0f : o / sum;
+      out[threadIdx.x] = kv_from<T>(o);
+      bad = !isfinite(o);
+    }
+    bad = __syncthreads_or(bad) && warp == 0;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float f[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = 128 * k + 4 * lane + e;
+        if (x < d) {
+          const float o = l == 0.0f ? 0.0f : f[e] / l;
+          out[x] = kv_from<T>(o);
+          bad |= !isfinite(o);
+        }
+      }
+    }
+    bad = __any_sync(0xffffffffu, bad);
   }
   // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
-  if (__syncthreads_or(bad) && warp == 0) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
+  if (bad) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
+  if constexpr (R == 1) __syncthreads();
+  }
 }
 
 // CTAs of a kernel that fit the GPU at once, remembered per device and kernel.
@@ -71,7 +154,7 @@ static int resident_ctas(const void* fn, int threads, size_t smem) {
       cudaGetLastError();
       per = 0;
     }
-    e = std::max(1, per) * std::max(1, sm_count());
+    e = std::min(std::max(1, per) * std::max(1, sm_count()), kMostCtas);
   }
   return e;
 }
@@ -83,6 +166,7 @@ struct KvLaunch {
   int rows_min = 0, rows_max = INT_MAX;
   size_t smem = 0;
   int ctas = 0;
+  bool one_per_sm = false;  // it takes all of an SM's tensor memory
   int merge_rows = 0;  // rows that an item of a call can have
 };
 
@@ -122,22 +206,40 @@ static KvLaunch mma_launch(int d, int rows) {
 // Rows of the pools are whole, aligned 16-byte chunks.
 static bool vector_rows(const KvView& c, size_t esize) { return c.d * esize % 16 == 0 && aligned16(c.k) && aligned16(c.v); }
 
-// The launches of a call, each over its class of sequences.
+// Query rows of a sequence's kv head up to which the warp-level kernel takes
+// it where both can: above, its 16- and 32-row items read the keys again and
+// again; below, 128-row tiles are mostly empty.
+constexpr int kFewRows = 32;
+
+// The launches of a call, each over its class of sequences.  one_each: every
+// sequence has one new token; qvec: rows of q are whole 16-byte chunks.
 template <typename T>
-static int pick(const KvView& c, int tokens, int n, int q_heads, KvLaunch (&out)[2]) {
+static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, bool qvec, KvLaunch (&out)[2]) {
   const int group = q_heads / c.hk;
-  const int rows = tokens <= n ? group : INT_MAX;
-  if constexpr (sizeof(T) == 2) {
-    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, rows) : scalar_launch<T>(c.d, rows);
+  const int most = one_each ? group : tokens * group;                 // rows that a sequence can have
+  const int likely = tokens <= n ? std::min(group, most) : most;      // and those to choose a shape by
+  int count = 1;
+  if (sizeof(T) == 2 && vector_rows(c, sizeof(T))) {
+    const bool tile = (c.d == 64 || c.d == 128) && qvec && tokens > n && most > kFewRows && is_sm100();
+    if constexpr (sizeof(T) == 2) {
+      out[0] = mma_launch<T>(c.d, tile ? kFewRows : likely);
+      if (tile) {
+        out[0].rows_max = kFewRows;
+        auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile_kernel<decltype(k)>, 2); };
+        out[1] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
+        out[1].rows_min = kFewRows;
+        out[1].one_per_sm = true;
+        count = 2;
+      }
+    }
   } else {
-    out[0] = scalar_launch<T>(c.d, rows);
+    out[0] = scalar_launch<T>(c.d, likely);
   }
-  const int count = 1;
   for (int i = 0; i < count; ++i) {
     const void* fn = reinterpret_cast<const void*>(out[i].kern);
     smem_attr_once(fn, out[i].smem);  // before the occupancy is asked for
-    out[i].ctas = resident_ctas(fn, out[i].threads, out[i].smem);
-    out[i].merge_rows = std::min(out[i].br, rows);
+    out[i].ctas = out[i].one_per_sm ? std::max(1, sm_count()) : resident_ctas(fn, out[i].threads, out[i].smem);
+    out[i].merge_rows = std::min(out[i].br, std::min(most, out[i].rows_max));
   }
   return count;
 }
@@ -149,9 +251,9 @@ static size_t workspace_floats(const KvLaunch* l, int count) {
 }
 
 template <typename T>
-static int run(KvAttn a, int q_heads, void* ws, size_t ws_bytes, cudaStream_t s) {
+static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, cudaStream_t s) {
   KvLaunch l[2];
-  const int count = pick<T>(a.c, a.bt.total, a.bt.n, q_heads, l);
+  const int count = pick<T>(a.c, a.bt.total, a.bt.n, q_heads, one_each, a.qvec, l);
   OC_REQUIRE(ws && aligned16(ws) && ws_bytes >= workspace_floats(l, count) * sizeof(float),
              "kv_attention: workspace too small or not 16-byte aligned");
   for (int i = 0; i < count; ++i) {
@@ -162,7 +264,13 @@ static int run(KvAttn a, int q_heads, void* ws, size_t ws_bytes, cudaStream_t s)
       return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
     OC_CHECK_CUDA(launch_pdl_ex(l[i].kern, dim3(l[i].ctas), dim3(l[i].threads), l[i].smem, s, a));
     if (l[i].ctas > 1)
-      OC_CHECK_CUDA(launch_pdl_ex(kv_merge_kernel<T>, dim3(l[i].ctas - 1, l[i].merge_rows), dim3(128), 0, s, a, l[i].dp));
+{
+      const bool few = l[i].merge_rows <= 16;
+      const int groups = few ? l[i].merge_rows : (l[i].merge_rows + 7) / 8;
+      const int64_t tasks = (int64_t)(l[i].ctas - 1) * groups;
+      const int grid = (int)std::min<int64_t>(tasks, 4 * (int64_t)std::max(1, sm_count()));
+      OC_CHECK_CUDA(launch_pdl_ex(few ? kv_merge_kernel<T, 1> : kv_merge_kernel<T, 8>, dim3(grid), dim3(256), 0, s, a, l[i].dp, groups));
+    }
   }
   return OC_OK;
 }
@@ -185,11 +293,16 @@ int oc_kv_attention_workspace_size(const oc_kv_cache* cache, int tokens, int n, 
   KvView c;
   if (int rc = attn_args(cache, &c, tokens, n, q_heads)) return rc;
   OC_REQUIRE(bytes, "kv_attention: NULL pointer");
-  KvLaunch l[2];
-  const int count = cache->dtype == OC_KV_F32   ? pick<float>(c, tokens, n, q_heads, l)
-                    : cache->dtype == OC_KV_F16 ? pick<__half>(c, tokens, n, q_heads, l)
-                                                : pick<__nv_bfloat16>(c, tokens, n, q_heads, l);
-  *bytes = workspace_floats(l, count) * sizeof(float);
+  size_t most = 0;
+  for (int form = 0; form < 4; ++form) {  // whatever cu and the alignment of q will be
+    KvLaunch l[2];
+    const bool one_each = form & 1, qvec = form & 2;
+    const int count = cache->dtype == OC_KV_F32   ? pick<float>(c, tokens, n, q_heads, one_each, qvec, l)
+                      : cache->dtype == OC_KV_F16 ? pick<__half>(c, tokens, n, q_heads, one_each, qvec, l)
+                                                  : pick<__nv_bfloat16>(c, tokens, n, q_heads, one_each, qvec, l);
+    most = std::max(most, workspace_floats(l, count));
+  }
+  *bytes = most * sizeof(float);
   return OC_OK;
 }
 
@@ -219,13 +332,14 @@ int oc_kv_attention(const oc_kv_cache* cache, int layer, int tokens, int n, cons
   a.scale2 = scale * 1.44269504088896341f;
   a.vec = vector_rows(c, es);
   a.qvec = c.d * es % 16 == 0 && aligned16(q) && q_stride * es % 16 == 0;
+  a.ovec16 = c.d * es % 16 == 0 && aligned16(out) && out_stride * es % 16 == 0;
   a.ovec = c.d % 2 == 0 && reinterpret_cast<uintptr_t>(out) % (2 * es) == 0 && out_stride % 2 == 0;
   a.ws = nullptr;
   a.dev_status = device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == OC_KV_F32) return run<float>(a, q_heads, workspace, workspace_bytes, s);
-  if (cache->dtype == OC_KV_F16) return run<__half>(a, q_heads, workspace, workspace_bytes, s);
-  return run<__nv_bfloat16>(a, q_heads, workspace, workspace_bytes, s);
+  if (cache->dtype == OC_KV_F32) return run<float>(a, q_heads, cu == nullptr, workspace, workspace_bytes, s);
+  if (cache->dtype == OC_KV_F16) return run<__half>(a, q_heads, cu == nullptr, workspace, workspace_bytes, s);
+  return run<__nv_bfloat16>(a, q_heads, cu == nullptr, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"

@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
         }
       } else {
         if (e == 0) slot[r] = mm, slot[ROWS + r] = ls;
-        *reinterpret_cast<float2*>(slot + 2 * ROWS + (size_t)r * DP + e) = os;
+        *reinterpret_cast<float2*>(slot + plan_slot_o(ROWS) + (size_t)r * DP + e) = os;
       }
     }
     if (__syncthreads_or(bad != 0)) {

@@ -208,9 +208,11 @@ struct KvCut {
   int b, h, r0, rows, q0, unused0, unused1;
 };
 
-// Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp], f32;
+// Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp]
+// (16-byte aligned), f32;
 // in front of them the cuts, one per CTA.
-__host__ __device__ inline size_t plan_slot_floats(int br, int dp) { return (size_t)br * (dp + 2); }
+__host__ __device__ inline size_t plan_slot_o(int br) { return (2 * (size_t)br + 3) / 4 * 4; }  // where o begins
+__host__ __device__ inline size_t plan_slot_floats(int br, int dp) { return plan_slot_o(br) + (size_t)br * dp; }
 __host__ __device__ inline size_t plan_cut_floats(int ctas) { return (size_t)ctas * (sizeof(KvCut) / sizeof(float)); }
 
 struct KvAttn {
@@ -224,6 +226,7 @@ struct KvAttn {
   float scale2;  // scale * log2(e)
   int vec;       // rows of the pools are whole 16-byte chunks
   int qvec;      // rows of q are
+  int ovec16;    // rows of out are whole 16-byte chunks
   int ovec;      // pairs of elements of out are 4-byte aligned
   float* ws;
   int* dev_status;

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
               kv_from<T>(ls == 0.0f ? 0.0f : os / ls);
       } else {
         if (e == 0) slot[r] = mm, slot[ROWS + r] = ls;
-        slot[2 * ROWS + (size_t)r * DP + e] = os;
+        slot[plan_slot_o(ROWS) + (size_t)r * DP + e] = os;
       }
     }
     __syncthreads();

@@ -162,6 +162,27 @@ def test_mixed_batch(dtype, d):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_fewer_tokens_than_sequences(dtype, d):
+    """One sequence has several new tokens, the others none."""
+    check(dtype, 8, 2, d, 32, [30, 20, 9000, 77, 1, 15], [0, 0, 5, 0, 0, 0], seed=d)
+    check(dtype, 8, 2, d, 32, [9000], [9], seed=d)
+    check(dtype, 8, 2, d, 32, [9000, 40], [9, 1], seed=d)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq, hk", [(1, 1), (7, 1), (8, 2), (9, 3), (40, 1)])
+def test_tiles_of_every_shape(dtype, d, hq, hk):
+    """Items with one sub-tile and two, with one tile of keys and many, cut and whole."""
+    for lens, new in (([33], [33]), ([128], [128]), ([129, 127], [129, 127]), ([256], [256]), ([257, 4000], [257, 130]), ([5000], [600]),
+                      ([6000, 70, 300, 2000, 1], [40, 70, 299, 1000, 1])):
+        check(dtype, hq, hk, d, 16, lens, new, seed=sum(lens))
+        check(dtype, hq, hk, d, 16, lens, new, seed=sum(lens), window=150)
+        check(dtype, hq, hk, d, 16, lens, new, seed=sum(lens), causal=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_many_short_sequences(dtype):
     lens = [1 + (7 * i) % 50 for i in range(400)]
     check(dtype, 4, 2, 64, 16, lens, [1] * 400, one_each=True)
