@@ -162,6 +162,8 @@ static int resident_ctas(const void* fn, int threads, size_t smem) {
 // One launch over a class of the batch's sequences: the kernel, its shape.
 struct KvLaunch {
   void (*kern)(KvAttn) = nullptr;
+  void (*tile)(KvAttn, CUtensorMap, CUtensorMap, int) = nullptr;  // or this one
+  const void* fn() const { return kern ? reinterpret_cast<const void*>(kern) : reinterpret_cast<const void*>(tile); }
   int br = 0, bk = 0, dp = 0, threads = 0, min_units = 1;
   int rows_min = 0, rows_max = INT_MAX;
   size_t smem = 0;
@@ -225,7 +227,11 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
       out[0] = mma_launch<T>(c.d, tile ? kFewRows : likely);
       if (tile) {
         out[0].rows_max = kFewRows;
-        auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile_kernel<decltype(k)>, 2); };
+        auto go = [](auto k) {
+          KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
+          l.tile = kv_tile_kernel<decltype(k)>;
+          return l;
+        };
         out[1] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
         out[1].rows_min = kFewRows;
         out[1].one_per_sm = true;
@@ -236,7 +242,7 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
     out[0] = scalar_launch<T>(c.d, likely);
   }
   for (int i = 0; i < count; ++i) {
-    const void* fn = reinterpret_cast<const void*>(out[i].kern);
+    const void* fn = out[i].fn();
     smem_attr_once(fn, out[i].smem);  // before the occupancy is asked for
     out[i].ctas = out[i].one_per_sm ? std::max(1, sm_count()) : resident_ctas(fn, out[i].threads, out[i].smem);
     out[i].merge_rows = std::min(out[i].br, std::min(most, out[i].rows_max));
@@ -260,9 +266,21 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
     a.p.br = l[i].br, a.p.bk_shift = __builtin_ctz(l[i].bk), a.p.rows_min = l[i].rows_min, a.p.rows_max = l[i].rows_max;
     a.p.ctas = l[i].ctas, a.p.min_units = l[i].min_units;
     a.ws = static_cast<float*>(ws);
-    if (!smem_attr_once(reinterpret_cast<const void*>(l[i].kern), l[i].smem))
-      return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
-    OC_CHECK_CUDA(launch_pdl_ex(l[i].kern, dim3(l[i].ctas), dim3(l[i].threads), l[i].smem, s, a));
+    if (!smem_attr_once(l[i].fn(), l[i].smem)) return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
+    const dim3 grid(l[i].ctas), block(l[i].threads);
+    if (l[i].kern) {
+      OC_CHECK_CUDA(launch_pdl_ex(l[i].kern, grid, block, l[i].smem, s, a));
+    } else {
+      // the pools as matrices of head_dim columns; a box is a page, or a tile of a larger one
+      const KvView& c = a.c;
+      const uint64_t rows = ((uint64_t)c.layers * c.pages * c.hk) << c.ps_shift;
+      const int box = c.ps_shift < 3 || rows > INT_MAX ? 0 : std::min(1 << c.ps_shift, l[i].bk);
+      CUtensorMap m[2] = {};
+      for (int x = 0; box && x < 2; ++x)
+        if (int rc = make_tmap_2d(&m[x], x ? c.v : c.k, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(T), c.d, rows, (uint64_t)c.d * sizeof(T), 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+          return rc;
+      OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], box));
+    }
     if (l[i].ctas > 1)
 {
       const bool few = l[i].merge_rows <= 16;

@@ -18,9 +18,12 @@
 //
 // 384 threads, one CTA an SM:
 //   warp 0       TMEM allocator, MMA issuer (lane 0)
-//   warps 1..3   loaders: rows of pages -> 128-byte-swizzled tiles by
-//                cp.async (a page of any size, even one token, is a list of
-//                rows), two stages each of K and V
+//   warps 1, 2   loaders of K and of V into 128-byte-swizzled tiles, two
+//                stages each: a tile whose keys are all there is a few TMA
+//                boxes (a page and 64 features each, one a lane); tiles at the
+//                ends, and pages of fewer than 8 tokens, are rows by cp.async,
+//                zeros in place of the keys that no row sees
+//   warp 3       loader of the item's queries
 //   warps 4..7   softmax and output of rows 0..127: thread = row = TMEM lane
 //   warps 8..11  the same of rows 128..255
 // Tensor memory: S / P of the two sub-tiles [0, 128) and [128, 256), O
@@ -41,7 +44,6 @@ template <typename T_, int D_>
 struct KvTile {
   using T = T_;
   static constexpr int D = D_, DP = D_, ROWS = 256, BK = 128, THREADS = 384;
-  static constexpr int LOADERS = 3;
   static constexpr int PANEL = 128 * 128;        // bytes of 64 features of 128 rows
   static constexpr int TILE = 128 * D * 2;       // bytes of 128 rows
   static constexpr int S_COL = 0, O_COL = 256, TMEM_COLS = 512;
@@ -60,6 +62,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
+__device__ __forceinline__ float kv_max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
 // The pieces of a CTA's run, walked alike by every role.
 struct KvWalk {
   KvCursor cur;
@@ -72,20 +80,82 @@ struct KvWalk {
   }
 };
 
-// Row `r` (lane's share) of a 128-row tile: 16-byte chunks.  D / 8 lanes take
-// a row, so a warp takes RPI rows an instruction.
+// 16-byte chunks of a 128-row tile: D / 8 lanes take a row, so a warp copies
+// RPI rows an instruction.
 template <typename K>
 struct KvTileRows {
-  static constexpr int LPR = K::D / 8, RPI = 32 / LPR, STEPS = 128 / RPI;
-  static constexpr int MINE = (STEPS + K::LOADERS - 1) / K::LOADERS;  // instructions of one loader warp
-  static constexpr int HELD = (MINE * RPI + 31) / 32;                 // offsets a lane keeps
+  static constexpr int LPR = K::D / 8, RPI = 32 / LPR;
   static __device__ __forceinline__ uint32_t off(int row, int chunk) {
     return (uint32_t)((chunk >> 3) * K::PANEL) + sw128_off(row, chunk & 7);
   }
 };
 
+// One warp: the K or the V tiles of a run.  `box`: keys a TMA box holds, 0
+// for pages that are too small.
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
+__device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CUtensorMap* map, const typename K::T* pool,
+                                             uint8_t* tiles, uint64_t* full, uint64_t* empty, int box, volatile int* abort_flag) {
+  using T = typename K::T;
+  using R = KvTileRows<K>;
+  const KvView& c = a.c;
+  const int lane = threadIdx.x & 31, my_row = lane / R::LPR, ch = lane % R::LPR;
+  uint32_t n = 0;
+  while (w.left > 0) {
+    const KvItem& it = w.cur.it;
+    const int t0 = w.first(), t1 = w.last();
+    const int* row = c.table + (size_t)max(w.cur.s.s, 0) * c.max_pages;
+    // boxes of a tile: one per `box` keys and 64 features; lane b has box b
+    // (there are at most 32: 128 keys in boxes of 8, two halves)
+    constexpr int PANELS = K::D / 64;
+    const int boxes = box ? PANELS * (K::BK / box) : 0;
+    const int my_key = box ? (lane / PANELS) * box : 0, my_panel = lane % PANELS;
+    auto page_of = [&](int t) {  // of this lane's box; -1: the tile goes row by row
+      const int key = (it.tile0 + t) * K::BK;
+      if (!box || key < it.lo || key + K::BK > it.hi) return -1;
+      if (lane >= boxes) return 0;
+      const int page = row[(key + my_key) >> c.ps_shift];
+      return page >= 0 && page < c.pages ? page : -1;
+    };
+    int page = page_of(t0);
+    for (int t = t0; t < t1; ++t, ++n) {
+      const uint32_t st = n & 1;
+      uint8_t* dst = tiles + st * K::TILE;
+      const int next = t + 1 < t1 ? page_of(t + 1) : -1;  // asked for before the wait
+      const int key0 = (it.tile0 + t) * K::BK;
+      if (!warp_wait(&empty[st], ((n >> 1) & 1) ^ 1, abort_flag)) return false;
+      if (__all_sync(0xffffffffu, page >= 0)) {
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], K::TILE);
+        __syncwarp();
+        if (lane < boxes) {
+          const int y = (int)(a.layer_off / K::D) + (int)((((int64_t)page * c.hk + w.cur.h) << c.ps_shift) +
+                                                          ((key0 + my_key) & ((1 << c.ps_shift) - 1)));
+          tma_load_2d(dst + my_panel * K::PANEL + my_key * 128, map, my_panel * 64, y, &full[st]);
+        }
+      } else {
+#pragma unroll 1
+        for (int x = 0; x < 128; x += 32) {
+          const int64_t off = kv_row_off(a, w.cur.s.s, w.cur.h, key0 + x + lane, it.lo, it.hi);
+#pragma unroll 4
+          for (int y = 0; y < 32; y += R::RPI) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, y + my_row);
+            cp_async16_zfill(dst + R::off(x + y + my_row, ch), pool + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+          }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+      }
+      page = next;
+    }
+    w.next(a, t1 - t0);
+  }
+  return true;
+}
+
+template <typename K>
+__global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, int box) {
   using T = typename K::T;
   using R = KvTileRows<K>;
   constexpr int D = K::D;
@@ -110,12 +180,12 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
   if (total == 0) return;
   w.left = min(chunk, total - chunk * blockIdx.x);
   if (threadIdx.x == 0) {
-    mbar_init(&bar.q_full, K::LOADERS);
+    mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], K::LOADERS);
+      mbar_init(&bar.k_full[i], 1);
       mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], K::LOADERS);
+      mbar_init(&bar.v_full[i], 1);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 1);
       mbar_init(&bar.p_full[i], 4);
@@ -197,105 +267,42 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
       }
       if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutMma);
     }
-  } else if (warp <= K::LOADERS) {
-    const int lw = warp - 1;
-    const T* kb = static_cast<const T*>(c.k) + a.layer_off;
-    const T* vb = static_cast<const T*>(c.v) + a.layer_off;
+  } else if (warp <= 2) {
+    const bool is_k = warp == 1;
+    if (box && lane == 0) prefetch_tmap(is_k ? &mk : &mv);
+    const T* pool = static_cast<const T*>(is_k ? c.k : c.v) + a.layer_off;
+    if (!kv_tile_load<K>(a, w, is_k ? &mk : &mv, pool, is_k ? sk : sv, is_k ? bar.k_full : bar.v_full,
+                         is_k ? bar.k_empty : bar.v_empty, box, abort_flag))
+      kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
+  } else if (warp == 3) {
     const int my_row = lane / R::LPR, ch = lane % R::LPR;
-    uint32_t n = 0, items = 0;
-    // copies in flight, oldest first: which barrier each group completes.  A
-    // group is announced two groups later (or at the end), when it has landed.
-    uint64_t *b0 = nullptr, *b1 = nullptr;
-    auto announce = [&](uint64_t* b) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b);
-    };
-    // Before this warp waits for room, what it has copied is announced: the
-    // consumers may need exactly that to make room.
-    auto take = [&](uint64_t* b, uint32_t parity) {
-      if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(b), parity))) return true;
-      cp_async_wait<0>();
-      if (b0) announce(b0);
-      if (b1) announce(b1);
-      b0 = b1 = nullptr;
-      return warp_wait(b, parity, abort_flag);
-    };
-    auto push = [&](uint64_t* b) {
-      cp_async_commit();
-      if (b0) {
-        cp_async_wait<2>();
-        announce(b0);
-      }
-      b0 = b1;
-      b1 = b;
-    };
-    bool ok = true;
-    while (ok && w.left > 0) {
+    for (uint32_t items = 0; w.left > 0; ++items) {
       const KvItem& it = w.cur.it;
-      const int t0 = w.first(), t1 = w.last();
-      // queries: rows of the item, zeros behind the last
-      ok = take(&bar.q_empty, (items & 1) ^ 1);
-      if (!ok) break;
+      if (!warp_wait(&bar.q_empty, (items & 1) ^ 1, abort_flag)) {
+        kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
+        break;
+      }
       const int q_rows = it.rows > 128 ? 256 : 128;
-      for (int r0 = lw * R::RPI; r0 < q_rows; r0 += K::LOADERS * R::RPI) {
+#pragma unroll 4
+      for (int r0 = 0; r0 < q_rows; r0 += R::RPI) {
         const int r = r0 + my_row, rr = it.r0 + r, token = plan_token(a.p, rr);
-        const bool there = r < it.rows;
+        const bool there = r < it.rows;  // zeros behind the last row
         const T* src = static_cast<const T*>(a.q);
         if (there) src += (int64_t)(w.cur.s.q0 + token) * a.qs + (int64_t)(w.cur.h * a.p.group + rr - token * a.p.group) * D + ch * 8;
         cp_async16_zfill(sq + (r >> 7) * K::TILE + R::off(r & 127, ch), src, there);
       }
-      push(&bar.q_full);
-      // offsets of this warp's rows of a tile: instruction i of the warp has
-      // rows (lw + LOADERS i) * RPI + lane / LPR; lane j keeps that of number j
-      int64_t off[R::HELD], nxt[R::HELD];
-      auto offsets = [&](int t, int64_t (&o)[R::HELD]) {
-#pragma unroll
-        for (int x = 0; x < R::HELD; ++x) {
-          const int j = x * 32 + lane, i = j / R::RPI;
-          const int row = (lw + K::LOADERS * i) * R::RPI + j % R::RPI;
-          o[x] = t < t1 && row < 128 ? kv_row_off(a, w.cur.s.s, w.cur.h, (it.tile0 + t) * K::BK + row, it.lo, it.hi) : -1;
-        }
-      };
-      auto copy = [&](const T* pool, uint8_t* dst) {
-#pragma unroll
-        for (int i = 0; i < R::MINE; ++i) {
-          const int step = lw + K::LOADERS * i;
-          const int64_t o = __shfl_sync(0xffffffffu, off[i * R::RPI / 32], (i * R::RPI) % 32 + my_row);
-          if (step < R::STEPS) cp_async16_zfill(dst + R::off(step * R::RPI + my_row, ch), pool + (o < 0 ? 0 : o) + ch * 8, o >= 0);
-        }
-      };
-      offsets(t0, off);
-      for (int t = t0; t < t1; ++t, ++n) {
-        const uint32_t st = n & 1, ph = ((n >> 1) & 1) ^ 1;
-        offsets(t + 1, nxt);
-        ok = take(&bar.k_empty[st], ph);
-        if (!ok) break;
-        copy(kb, sk + st * K::TILE);
-        push(&bar.k_full[st]);
-        ok = take(&bar.v_empty[st], ph);
-        if (!ok) break;
-        copy(vb, sv + st * K::TILE);
-        push(&bar.v_full[st]);
-#pragma unroll
-        for (int x = 0; x < R::HELD; ++x) off[x] = nxt[x];
-      }
-      ++items;
-      w.next(a, t1 - t0);
-    }
-    cp_async_wait<0>();
-    if (ok) {
-      if (b0) announce(b0);
-      if (b1) announce(b1);
-    } else {
-      kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.q_full);
+      w.next(a, w.last() - w.first());
     }
   } else {
     const int sub = (warp - 4) >> 2, quad = warp & 3, row = sub * 128 + quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t s_col = tmem + K::S_COL + sub * 128 + lanes, o_col = tmem + K::O_COL + sub * D + lanes;
-    const float sc = fabsf(a.scale2);
-    const bool flip = a.scale2 < 0.0f;
+    const float sc = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
     uint32_t ph = 0, od = 0;  // phases of s_full and of o_done (one each a tile)
     bool ok = true;
     while (ok && w.left > 0) {
@@ -312,8 +319,6 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
         float m = -INFINITY, l = 0.0f;  // log2 units
         for (int t = t0; t < t1; ++t) {
           const int key0 = (it.tile0 + t) * K::BK;
-          const bool masked = key0 < all_lo || key0 + K::BK > all_hi;
-          const int from = lo - key0, to = hi - key0;  // of this row, within the tile
           ok = warp_wait(&bar.s_full[sub], ph, abort_flag);
           ph ^= 1;
           if (!ok) break;
@@ -322,18 +327,26 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) tmem_ld32(s_col + x * 32, *reinterpret_cast<uint32_t(*)[32]>(s + x * 32));
           tmem_ld_wait();
-          if (flip)
+          if (a.scale2 <= 0.0f) {  // the sign goes to the scores; a scale of zero leaves zeros (and NaN of infinities)
+            const float by = a.scale2 < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
-            for (int x = 0; x < 128; ++x) s[x] ^= 0x80000000u;
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (masked) {
+            for (int x = 0; x < 128; ++x) s[x] = __float_as_uint(__uint_as_float(s[x]) * by);
+          }
+          if (key0 < all_lo || key0 + K::BK > all_hi) {
+            const int from = lo - key0, to = hi - key0;  // of this row, within the tile
 #pragma unroll
             for (int x = 0; x < 128; ++x)
-              if (x >= from && x < to) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
-          } else {
-#pragma unroll
-            for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x]));
+              if (x < from || x >= to) s[x] = 0xff800000u;  // minus infinity
           }
+          float mx[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
+#pragma unroll
+          for (int x = 4; x < 124; x += 8)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) mx[y] = kv_max3(mx[y], __uint_as_float(s[x + 2 * y]), __uint_as_float(s[x + 2 * y + 1]));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], __uint_as_float(s[124 + y]));
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const float mn = top == -INFINITY ? m : fmaxf(m, top * sc);
           if (__any_sync(0xffffffffu, mn > m + 8.0f)) {
@@ -358,28 +371,27 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a) {
             }
           }
           const float nb = m == -INFINITY ? 0.0f : -m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          auto weigh = [&](int x) {
-            const float p = kv_ex2(fmaf(__uint_as_float(s[x]), sc, nb));
-            return p;
-          };
+          const uint64_t sc2 = f2_pack(sc, sc), nb2 = f2_pack(nb, nb);
+          uint64_t sum2[2] = {0, 0};  // two pairs of f32 zeros
 #pragma unroll
           for (int x0 = 0; x0 < 128; x0 += 32) {
             uint32_t p[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              float p0 = weigh(x0 + x), p1 = weigh(x0 + x + 1);
-              if (masked) {
-                p0 = x0 + x >= from && x0 + x < to ? p0 : 0.0f;
-                p1 = x0 + x + 1 >= from && x0 + x + 1 < to ? p1 : 0.0f;
-              }
-              sum[x & 2] += p0;
-              sum[(x & 2) + 1] += p1;
+              float p0, p1;
+              f2_unpack(f2_fma(u2_pack(s[x0 + x], s[x0 + x + 1]), sc2, nb2), p0, p1);
+              p0 = kv_ex2(p0);
+              p1 = kv_ex2(p1);
+              sum2[(x >> 1) & 1] = f2_add(sum2[(x >> 1) & 1], f2_pack(p0, p1));
               p[x >> 1] = kv_pack2<T>(p0, p1);
             }
             tmem_st16(s_col + x0 / 2, p);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          {
+            float x0, x1;
+            f2_unpack(f2_add(sum2[0], sum2[1]), x0, x1);
+            l += x0 + x1;
+          }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
