@@ -19,10 +19,10 @@
 // 384 threads, one CTA an SM:
 //   warp 0       TMEM allocator, MMA issuer (lane 0)
 //   warps 1, 2   loaders of K and of V into 128-byte-swizzled tiles, two
-//                stages each: a tile whose keys are all there is a few TMA
-//                boxes (a page and 64 features each, one a lane); tiles at the
-//                ends, and pages of fewer than 8 tokens, are rows by cp.async,
-//                zeros in place of the keys that no row sees
+//                stages each: a tile whose keys the sequence holds is a few
+//                TMA boxes (a page and 64 features each, one a lane); its last
+//                tile, and pages of fewer than 8 tokens, are rows by cp.async,
+//                zeros in place of keys that are not there
 //   warp 3       loader of the item's queries
 //   warps 4..7   softmax and output of rows 0..127: thread = row = TMEM lane
 //   warps 8..11  the same of rows 128..255
@@ -54,7 +54,7 @@ struct KvTile {
 
 struct KvTileBars {
   uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
+  uint64_t s_full[2], p_part[2], p_full[2], o_done[2], o_free[2];
 };
 
 // mbar_wait of a whole warp: all lanes go on, or all give up.
@@ -111,7 +111,7 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CU
     const int my_key = box ? (lane / PANELS) * box : 0, my_panel = lane % PANELS;
     auto page_of = [&](int t) {  // of this lane's box; -1: the tile goes row by row
       const int key = (it.tile0 + t) * K::BK;
-      if (!box || key < it.lo || key + K::BK > it.hi) return -1;
+      if (!box || key + K::BK > w.cur.s.len) return -1;
       if (lane >= boxes) return 0;
       const int page = row[(key + my_key) >> c.ps_shift];
       return page >= 0 && page < c.pages ? page : -1;
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
       mbar_init(&bar.v_full[i], 1);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_part[i], 4);
       mbar_init(&bar.p_full[i], 4);
       mbar_init(&bar.o_done[i], 1);
       mbar_init(&bar.o_free[i], 4);
@@ -237,15 +238,22 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
               ok = mbar_wait(&bar.o_free[s], of_ph[s], abort_flag);
               of_ph[s] ^= 1;
             }
-            ok = ok && mbar_wait(&bar.p_full[s], p_ph[s], abort_flag);
-            p_ph[s] ^= 1;
+            ok = ok && mbar_wait(&bar.p_part[s], p_ph[s], abort_flag);
             if (!ok) break;
             tc_fence_after();
             const uint32_t v0 = smem_u32(sv) + (n & 1) * K::TILE;
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
+            auto product = [&](int kk) {  // 16 keys
               mma_f16_ta(tmem + K::O_COL + s * D, tmem + K::S_COL + s * 128 + kk * 8,
                          desc_mnmajor_sw128(v0 + kk * 2048, K::PANEL, 1024), idesc_o, t != 0 || kk != 0);
+            };
+#pragma unroll
+            for (int kk = 0; kk < 6; ++kk) product(kk);
+            ok = mbar_wait(&bar.p_full[s], p_ph[s], abort_flag);
+            p_ph[s] ^= 1;
+            if (!ok) break;
+            tc_fence_after();
+            product(6);
+            product(7);
             tc_commit(&bar.o_done[s]);
             if (s == subs - 1) tc_commit(&bar.v_empty[n & 1]);
             if (more) {
@@ -386,6 +394,12 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
               p[x >> 1] = kv_pack2<T>(p0, p1);
             }
             tmem_st16(s_col + x0 / 2, p);
+            if (x0 == 64) {  // three quarters of the product may begin
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar.p_part[sub]);
+            }
           }
           {
             float x0, x1;
