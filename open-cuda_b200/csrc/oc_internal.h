@@ -48,6 +48,12 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
                  uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
                  CUtensorMapSwizzle swizzle);
 
+// The same for [planes][rows][cols] with a stride for each of the two outer
+// dimensions and a box {box_cols, box_rows, box_planes}.
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t cols, uint64_t rows,
+                 uint64_t row_stride_bytes, uint64_t planes, uint64_t plane_stride_bytes, uint32_t box_cols,
+                 uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle);
+
 // Device-side status word per device: kernels write a nonzero code there
 // instead of trapping (bounded waits that expired, bad indices).
 int* device_status_word();

@@ -162,7 +162,7 @@ static int resident_ctas(const void* fn, int threads, size_t smem) {
 // One launch over a class of the batch's sequences: the kernel, its shape.
 struct KvLaunch {
   void (*kern)(KvAttn) = nullptr;
-  void (*tile)(KvAttn, CUtensorMap, CUtensorMap, int) = nullptr;  // or this one
+  void (*tile)(KvAttn, CUtensorMap, CUtensorMap, CUtensorMap, int, int) = nullptr;  // or this one
   const void* fn() const { return kern ? reinterpret_cast<const void*>(kern) : reinterpret_cast<const void*>(tile); }
   int br = 0, bk = 0, dp = 0, threads = 0, min_units = 1;
   int rows_min = 0, rows_max = INT_MAX;
@@ -275,11 +275,19 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
       const KvView& c = a.c;
       const uint64_t rows = ((uint64_t)c.layers * c.pages * c.hk) << c.ps_shift;
       const int box = c.ps_shift < 3 || rows > INT_MAX ? 0 : std::min(1 << c.ps_shift, l[i].bk);
-      CUtensorMap m[2] = {};
+      const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+      CUtensorMap m[3] = {};
       for (int x = 0; box && x < 2; ++x)
-        if (int rc = make_tmap_2d(&m[x], x ? c.v : c.k, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(T), c.d, rows, (uint64_t)c.d * sizeof(T), 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+        if (int rc = make_tmap_2d(&m[x], x ? c.v : c.k, type, sizeof(T), c.d, rows, (uint64_t)c.d * sizeof(T), 64, box,
+                                  CU_TENSOR_MAP_SWIZZLE_128B))
           return rc;
-      OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], box));
+      // the queries as [token][head][feature]: a box is all heads of a group, of 128 / G tokens
+      const int g = a.p.group, qbox = 128 % g == 0 ? 128 / g : 0;
+      if (qbox)
+        if (int rc = make_tmap_3d(&m[2], a.q, type, c.d, q_heads, (uint64_t)c.d * sizeof(T), a.bt.total, (uint64_t)a.qs * sizeof(T), 64, g,
+                                  qbox, CU_TENSOR_MAP_SWIZZLE_128B))
+          return rc;
+      OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], m[2], box, qbox));
     }
     if (l[i].ctas > 1)
 {

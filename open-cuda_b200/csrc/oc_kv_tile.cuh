@@ -23,7 +23,8 @@
 //                TMA boxes (a page and 64 features each, one a lane); its last
 //                tile, and pages of fewer than 8 tokens, are rows by cp.async,
 //                zeros in place of keys that are not there
-//   warp 3       loader of the item's queries
+//   warp 3       walks the CTA's run and hands its pieces to the others;
+//                loader of the queries (TMA where 128 rows are whole tokens)
 //   warps 4..7   softmax and output of rows 0..127: thread = row = TMEM lane
 //   warps 8..11  the same of rows 128..255
 // Tensor memory: S / P of the two sub-tiles [0, 128) and [128, 256), O
@@ -52,9 +53,18 @@ struct KvTile {
   static constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
 };
 
+// A piece of an item: its tiles [t0, t1) of `units`.  One warp walks the
+// CTA's run and hands the pieces to the others, a few ahead.
+struct KvJob {
+  KvSeq s;
+  int b, h, r0, rows, lo, hi, tile0, units, t0, t1;  // t0 == t1: the run is over
+};
+constexpr int kJobs = 4;
+
 struct KvTileBars {
   uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_part[2], p_full[2], o_done[2], o_free[2];
+  uint64_t job_full[kJobs], job_empty[kJobs];
 };
 
 // mbar_wait of a whole warp: all lanes go on, or all give up.
@@ -68,15 +78,24 @@ __device__ __forceinline__ float kv_max3(float x, float y, float z) {
   return r;
 }
 
-// The pieces of a CTA's run, walked alike by every role.
-struct KvWalk {
-  KvCursor cur;
-  int64_t left;
-  __device__ __forceinline__ int first() const { return cur.at; }
-  __device__ __forceinline__ int last() const { return (int)min((int64_t)cur.it.units, cur.at + left); }
-  __device__ __forceinline__ void next(const KvAttn& a, int done) {
-    left -= done;
-    if (left > 0) plan_next(a.p, a.c, a.bt, cur);
+// A consumer's place in the ring of jobs.
+struct KvJobs {
+  const KvJob* ring;
+  KvTileBars* bar;
+  uint32_t at = 0, phase = 0;
+  // The next job; false when a wait gave up.  Whole warps, or one thread.
+  template <bool WARP>
+  __device__ __forceinline__ bool take(KvJob& j, volatile int* abort_flag) {
+    const bool ok = WARP ? warp_wait(&bar->job_full[at], phase, abort_flag) : mbar_wait(&bar->job_full[at], phase, abort_flag);
+    if (ok) j = ring[at];
+    return ok;
+  }
+  // Done with it.
+  template <bool WARP>
+  __device__ __forceinline__ void drop() {
+    if (WARP) __syncwarp();
+    if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&bar->job_empty[at]);
+    if (++at == kJobs) at = 0, phase ^= 1;
   }
 };
 
@@ -93,17 +112,19 @@ struct KvTileRows {
 // One warp: the K or the V tiles of a run.  `box`: keys a TMA box holds, 0
 // for pages that are too small.
 template <typename K>
-__device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CUtensorMap* map, const typename K::T* pool,
+__device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs jobs, const CUtensorMap* map, const typename K::T* pool,
                                              uint8_t* tiles, uint64_t* full, uint64_t* empty, int box, volatile int* abort_flag) {
   using T = typename K::T;
   using R = KvTileRows<K>;
   const KvView& c = a.c;
   const int lane = threadIdx.x & 31, my_row = lane / R::LPR, ch = lane % R::LPR;
   uint32_t n = 0;
-  while (w.left > 0) {
-    const KvItem& it = w.cur.it;
-    const int t0 = w.first(), t1 = w.last();
-    const int* row = c.table + (size_t)max(w.cur.s.s, 0) * c.max_pages;
+  for (;;) {
+    KvJob it;
+    if (!jobs.take<true>(it, abort_flag)) return false;
+    const int t0 = it.t0, t1 = it.t1;
+    if (t0 == t1) return true;
+    const int* row = c.table + (size_t)max(it.s.s, 0) * c.max_pages;
     // boxes of a tile: one per `box` keys and 64 features; lane b has box b
     // (there are at most 32: 128 keys in boxes of 8, two halves)
     constexpr int PANELS = K::D / 64;
@@ -111,7 +132,7 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CU
     const int my_key = box ? (lane / PANELS) * box : 0, my_panel = lane % PANELS;
     auto page_of = [&](int t) {  // of this lane's box; -1: the tile goes row by row
       const int key = (it.tile0 + t) * K::BK;
-      if (!box || key + K::BK > w.cur.s.len) return -1;
+      if (!box || key + K::BK > it.s.len) return -1;
       if (lane >= boxes) return 0;
       const int page = row[(key + my_key) >> c.ps_shift];
       return page >= 0 && page < c.pages ? page : -1;
@@ -127,14 +148,14 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CU
         if (lane == 0) mbar_arrive_expect_tx(&full[st], K::TILE);
         __syncwarp();
         if (lane < boxes) {
-          const int y = (int)(a.layer_off / K::D) + (int)((((int64_t)page * c.hk + w.cur.h) << c.ps_shift) +
+          const int y = (int)(a.layer_off / K::D) + (int)((((int64_t)page * c.hk + it.h) << c.ps_shift) +
                                                           ((key0 + my_key) & ((1 << c.ps_shift) - 1)));
           tma_load_2d(dst + my_panel * K::PANEL + my_key * 128, map, my_panel * 64, y, &full[st]);
         }
       } else {
 #pragma unroll 1
         for (int x = 0; x < 128; x += 32) {
-          const int64_t off = kv_row_off(a, w.cur.s.s, w.cur.h, key0 + x + lane, it.lo, it.hi);
+          const int64_t off = kv_row_off(a, it.s.s, it.h, key0 + x + lane, it.lo, it.hi);
 #pragma unroll 4
           for (int y = 0; y < 32; y += R::RPI) {
             const int64_t o = __shfl_sync(0xffffffffu, off, y + my_row);
@@ -149,19 +170,20 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvWalk w, const CU
       }
       page = next;
     }
-    w.next(a, t1 - t0);
+    jobs.drop<true>();
   }
-  return true;
 }
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, int box) {
+__global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                   const __grid_constant__ CUtensorMap mq, int box, int qbox) {
   using T = typename K::T;
   using R = KvTileRows<K>;
   constexpr int D = K::D;
   extern __shared__ uint8_t raw[];
   __shared__ KvPlanShared plan;
   __shared__ KvTileBars bar;
+  __shared__ KvJob ring[kJobs];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -173,12 +195,11 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
   pdl_wait();
   pdl_launch();
   const KvView& c = a.c;
-  KvWalk w;
+  KvCursor cur;
   int64_t chunk;
-  const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, w.cur);
+  const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, cur);
   if (threadIdx.x == 0) plan_no_cut(a);
   if (total == 0) return;
-  w.left = min(chunk, total - chunk * blockIdx.x);
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_empty, 1);
@@ -193,6 +214,10 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
       mbar_init(&bar.o_done[i], 1);
       mbar_init(&bar.o_free[i], 4);
     }
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(&bar.job_full[i], 1);
+      mbar_init(&bar.job_empty[i], 3 + 8);  // MMA issuer, two loaders, eight softmax warps
+    }
     abort_word = 0;
     fence_mbar_init();
   }
@@ -204,6 +229,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  KvJobs jobs{ring, &bar};
 
   if (warp == 0) {
     if (lane == 0) {
@@ -221,8 +247,11 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
         tc_commit(&bar.s_full[sub]);
       };
       bool ok = true;
-      while (ok && w.left > 0) {
-        const int tiles = w.last() - w.first(), subs = w.cur.it.rows > 128 ? 2 : 1;
+      for (;;) {
+        KvJob it;
+        ok = jobs.take<false>(it, abort_flag);
+        const int tiles = it.t1 - it.t0, subs = it.rows > 128 ? 2 : 1;
+        if (!ok || tiles == 0) break;
         ok = mbar_wait(&bar.q_full, items & 1, abort_flag) && mbar_wait(&bar.k_full[n & 1], (n >> 1) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -270,8 +299,9 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
             }
           }
         }
+        if (!ok) break;
         ++items;
-        w.next(a, tiles);
+        jobs.drop<false>();
       }
       if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutMma);
     }
@@ -279,33 +309,59 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
     const bool is_k = warp == 1;
     if (box && lane == 0) prefetch_tmap(is_k ? &mk : &mv);
     const T* pool = static_cast<const T*>(is_k ? c.k : c.v) + a.layer_off;
-    if (!kv_tile_load<K>(a, w, is_k ? &mk : &mv, pool, is_k ? sk : sv, is_k ? bar.k_full : bar.v_full,
+    if (!kv_tile_load<K>(a, jobs, is_k ? &mk : &mv, pool, is_k ? sk : sv, is_k ? bar.k_full : bar.v_full,
                          is_k ? bar.k_empty : bar.v_empty, box, abort_flag))
       kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
   } else if (warp == 3) {
-    const int my_row = lane / R::LPR, ch = lane % R::LPR;
-    for (uint32_t items = 0; w.left > 0; ++items) {
-      const KvItem& it = w.cur.it;
-      if (!warp_wait(&bar.q_empty, (items & 1) ^ 1, abort_flag)) {
-        kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
-        break;
+    // walks the run: hands out each piece, then brings its queries
+    int64_t left = min(chunk, total - chunk * blockIdx.x);
+    if (qbox && lane == 0) prefetch_tmap(&mq);
+    bool ok = true;
+    for (uint32_t items = 0; ok; ++items) {
+      const uint32_t at = items % kJobs, ph = (items / kJobs) & 1;
+      ok = warp_wait(&bar.job_empty[at], ph ^ 1, abort_flag);
+      if (!ok) break;
+      const int t0 = cur.at, t1 = left > 0 ? (int)min((int64_t)cur.it.units, t0 + left) : t0;
+      if (lane == 0) {
+        ring[at] = KvJob{cur.s, cur.b, cur.h, cur.it.r0, cur.it.rows, cur.it.lo, cur.it.hi, cur.it.tile0, cur.it.units, t0, t1};
+        if (t0 == 0 && t0 < t1 && t1 < cur.it.units) plan_cut(a, cur, cur.it.units - t1, chunk);
+        mbar_arrive(&bar.job_full[at]);
       }
-      const int q_rows = it.rows > 128 ? 256 : 128;
+      if (t0 == t1) break;
+      ok = warp_wait(&bar.q_empty, (items & 1) ^ 1, abort_flag);
+      if (!ok) break;
+      const int subs = cur.it.rows > 128 ? 2 : 1;
+      if (qbox) {  // 128 rows are all heads of the group of 128 / G tokens (what lies behind the last row is not used)
+        if (lane == 0) mbar_arrive_expect_tx(&bar.q_full, subs * K::TILE);
+        __syncwarp();
+        if (lane < subs * (D / 64)) {
+          const int sub = lane / (D / 64), panel = lane % (D / 64);
+          tma_load_3d(sq + sub * K::TILE + panel * K::PANEL, &mq, panel * 64, cur.h * a.p.group,
+                      cur.s.q0 + plan_token(a.p, cur.it.r0) + sub * qbox, &bar.q_full);
+        }
+      } else {
+        const int my_row = lane / R::LPR, ch = lane % R::LPR;
+#pragma unroll 1
+        for (int x = 0; x < subs * 128; x += 32) {
+          const int r = x + lane, rr = cur.it.r0 + r, token = plan_token(a.p, rr);  // zeros behind the last row
+          const int64_t off = r < cur.it.rows ? (int64_t)(cur.s.q0 + token) * a.qs + (int64_t)(cur.h * a.p.group + rr - token * a.p.group) * D : -1;
 #pragma unroll 4
-      for (int r0 = 0; r0 < q_rows; r0 += R::RPI) {
-        const int r = r0 + my_row, rr = it.r0 + r, token = plan_token(a.p, rr);
-        const bool there = r < it.rows;  // zeros behind the last row
-        const T* src = static_cast<const T*>(a.q);
-        if (there) src += (int64_t)(w.cur.s.q0 + token) * a.qs + (int64_t)(w.cur.h * a.p.group + rr - token * a.p.group) * D + ch * 8;
-        cp_async16_zfill(sq + (r >> 7) * K::TILE + R::off(r & 127, ch), src, there);
+          for (int y = 0; y < 32; y += R::RPI) {
+            const int64_t o = __shfl_sync(0xffffffffu, off, y + my_row);
+            cp_async16_zfill(sq + (x >> 7) * K::TILE + R::off((x & 127) + y + my_row, ch), static_cast<const T*>(a.q) + (o < 0 ? 0 : o) + ch * 8,
+                             o >= 0);
+          }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.q_full);
       }
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.q_full);
-      w.next(a, w.last() - w.first());
+      left -= t1 - t0;
+      if (left > 0) plan_next(a.p, c, a.bt, cur);
     }
+    if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
   } else {
     const int sub = (warp - 4) >> 2, quad = warp & 3, row = sub * 128 + quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
@@ -313,17 +369,19 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
     const float sc = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2);
     uint32_t ph = 0, od = 0;  // phases of s_full and of o_done (one each a tile)
     bool ok = true;
-    while (ok && w.left > 0) {
-      const KvItem& it = w.cur.it;
-      const int t0 = w.first(), t1 = w.last();
+    for (;;) {
+      KvJob it;
+      ok = jobs.take<true>(it, abort_flag);
+      const int t0 = it.t0, t1 = it.t1;
+      if (!ok || t0 == t1) break;
       const bool active = it.rows > sub * 128;  // the whole warp group
       if (active) {
         int lo = 0, hi = 0;
-        if (row < it.rows) plan_row_range(a.p, w.cur.s, it.r0 + row, lo, hi);
+        if (row < it.rows) plan_row_range(a.p, it.s, it.r0 + row, lo, hi);
         // keys that all rows of the sub-tile see
         int all_lo, all_hi, unused;
-        plan_row_range(a.p, w.cur.s, it.r0 + sub * 128, unused, all_hi);
-        plan_row_range(a.p, w.cur.s, it.r0 + min(it.rows, sub * 128 + 128) - 1, all_lo, unused);
+        plan_row_range(a.p, it.s, it.r0 + sub * 128, unused, all_hi);
+        plan_row_range(a.p, it.s, it.r0 + min(it.rows, sub * 128 + 128) - 1, all_lo, unused);
         float m = -INFINITY, l = 0.0f;  // log2 units
         for (int t = t0; t < t1; ++t) {
           const int key0 = (it.tile0 + t) * K::BK;
@@ -420,8 +478,8 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
         if (whole) {
           const int rr = it.r0 + row, token = plan_token(a.p, rr);
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          T* out = static_cast<T*>(a.out) + (int64_t)(w.cur.s.q0 + token) * a.os +
-                   (int64_t)(w.cur.h * a.p.group + rr - token * a.p.group) * D;
+          T* out = static_cast<T*>(a.out) + (int64_t)(it.s.q0 + token) * a.os +
+                   (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D;
           bool bad = false;
 #pragma unroll 1
           for (int x = 0; x < D; x += 32) {
@@ -449,7 +507,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
           }
           __syncwarp();
           for (uint32_t todo = __ballot_sync(0xffffffffu, bad); todo; todo &= todo - 1)
-            kv_row_exact<T>(a, w.cur.s, w.cur.h, it.r0 + sub * 128 + quad * 32 + __ffs(todo) - 1);
+            kv_row_exact<T>(a, it.s, it.h, it.r0 + sub * 128 + quad * 32 + __ffs(todo) - 1);
         } else {
           float* slot = plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D);
           if (row < it.rows) slot[row] = m, slot[K::ROWS + row] = l;
@@ -469,8 +527,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.o_free[sub]);
       }
-      if (threadIdx.x == 128 && t0 == 0 && t1 < it.units) plan_cut(a, w.cur, it.units - t1, chunk);
-      w.next(a, t1 - t0);
+      jobs.drop<true>();
     }
     if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutEpilogue);
   }

@@ -124,9 +124,10 @@ bool smem_attr_once(const void* fn, size_t bytes) {
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 static std::once_flag g_encode_once;
 
-int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
-                 uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
-                 CUtensorMapSwizzle swizzle) {
+// Tiled map of rank 2 or 3 with element strides 1 (dims, strides in bytes of
+// dims 1.., box).
+static int encode_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   std::call_once(g_encode_once, [] {
     cudaDriverEntryPointQueryResult q;
     void* fn = nullptr;
@@ -135,22 +136,35 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (!g_encode) return fail(OC_ERR_NO_DEVICE, "cuTensorMapEncodeTiled unavailable");
-  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_stride_bytes & 15u) != 0)
-    return fail(OC_ERR_INVALID_VALUE, "tensor map: base and row stride must be 16-byte aligned");
-  (void)elem_bytes;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {row_stride_bytes};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  bool aligned = (reinterpret_cast<uintptr_t>(base) & 15u) == 0;
+  for (int i = 0; i + 1 < rank; ++i) aligned = aligned && (strides[i] & 15u) == 0;
+  if (!aligned) return fail(OC_ERR_INVALID_VALUE, "tensor map: base and row stride must be 16-byte aligned");
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, dtype, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     char buf[160];
     snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return fail(OC_ERR_INVALID_VALUE, buf);
   }
   return OC_OK;
+}
+
+int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
+                 uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
+                 CUtensorMapSwizzle swizzle) {
+  (void)elem_bytes;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_stride_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  return encode_tmap(map, base, dtype, 2, dims, strides, box, swizzle);
+}
+
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t cols, uint64_t rows,
+                 uint64_t row_stride_bytes, uint64_t planes, uint64_t plane_stride_bytes, uint32_t box_cols,
+                 uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {row_stride_bytes, plane_stride_bytes};
+  const cuuint32_t box[3] = {box_cols, box_rows, box_planes};
+  return encode_tmap(map, base, dtype, 3, dims, strides, box, swizzle);
 }
 
 }  // namespace oc
