@@ -9,6 +9,16 @@ namespace oc {
 
 constexpr int kMostCtas = 2048;  // of an attention kernel's grid
 
+// The partial results of one launch.
+struct KvPart {
+  float* ws;
+  int ctas, br, groups;  // groups: of R rows, that an item can have
+};
+struct KvParts {
+  KvPart of[2];
+  int count;
+};
+
 // Joins the pieces of the items that cuts went through.  R rows of an item at
 // a time: one, its pieces shared by the 8 warps, for decode steps, where an
 // item of a long sequence has few rows and dozens of pieces; eight, a warp
@@ -17,126 +27,137 @@ constexpr int kMostCtas = 2048;  // of an attention kernel's grid
 // row costs one trip to memory.  Every CTA lists the cuts that went through
 // an item and takes its share of their rows: a CTA per possible cut and row
 // would mostly be launched to find nothing (2065 CTAs, 8 us, at 296 x 7).
-template <typename T, int R>
-__global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, int dp, int groups) {
-  constexpr int WARPS = 8, SPLIT = WARPS / R;  // warps that share a row
-  __shared__ float part[R == 1 ? WARPS : 1][256], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
-  __shared__ unsigned short list[kMostCtas];
+// DP: features of a row, 128 or 256.
+template <typename T, int R, int DP>
+__global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, KvParts parts, int dp) {
+  constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
+  __shared__ float part[R == 1 ? WARPS : 1][DP], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
+  __shared__ unsigned short list[2][kMostCtas];
   __shared__ int wcount[WARPS];
   const KvView& c = a.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, br = a.p.br, d = c.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = c.d;
   pdl_wait();
-  const KvCut* cuts = reinterpret_cast<const KvCut*>(a.ws);
-  int found = 0;
-  for (int i0 = 0; i0 < a.p.ctas; i0 += 256) {
-    const int i = i0 + threadIdx.x;
-    const bool there = i < a.p.ctas && cuts[i].pieces > 0;
-    const uint32_t votes = __ballot_sync(0xffffffffu, there);
-    if (lane == 0) wcount[warp] = __popc(votes);
-    __syncthreads();
-    int at = found;
+  int found[2] = {0, 0};
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) at += wcount[w];
-      found += wcount[w];
-    }
-    if (there) list[at + __popc(votes & ((1u << lane) - 1))] = (unsigned short)i;
-    __syncthreads();
-  }
-  for (int task = blockIdx.x; task < found * groups; task += gridDim.x) {
-  const int cta = list[task / groups];
-  const KvCut cut = cuts[cta];
-  const int pieces = cut.pieces, r = (task % groups) * R + warp / SPLIT;
-  if (r >= cut.rows) continue;  // R == 1: the whole CTA; else the warp has nobody to meet
-  const size_t step = 2 * plan_slot_floats(br, dp);
-  // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
-  const float* first = plan_slot(a, cta, 1, dp);
-  const float* rest = plan_slot(a, cta + 1, 0, dp);
-  constexpr int U = 4;
-  float m = -INFINITY, l = 0.0f;
-  float4 acc[2] = {};  // features 4 lane .. and 128 + 4 lane ..
-  for (int i0 = warp % SPLIT; i0 < pieces; i0 += SPLIT * U) {
-    float pm[U], pl[U];
-    float4 po[U][2];
+  for (int k = 0; k < 2; ++k) {
+    if (k >= parts.count) break;
+    const KvCut* cuts = reinterpret_cast<const KvCut*>(parts.of[k].ws);
+    for (int i0 = 0; i0 < parts.of[k].ctas; i0 += 256) {
+      const int i = i0 + threadIdx.x;
+      const bool there = i < parts.of[k].ctas && cuts[i].pieces > 0;
+      const uint32_t votes = __ballot_sync(0xffffffffu, there);
+      if (lane == 0) wcount[warp] = __popc(votes);
+      __syncthreads();
+      int at = found[k];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * SPLIT;
-      pm[u] = -INFINITY, pl[u] = 0.0f;
-      po[u][0] = po[u][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i < pieces) {
-        const float* s = i == 0 ? first : rest + (size_t)(i - 1) * step;
-        const float* o = s + plan_slot_o(br) + (size_t)r * dp;
-        pm[u] = s[r];
-        pl[u] = s[br + r];
-        if (4 * lane < dp) po[u][0] = *reinterpret_cast<const float4*>(o + 4 * lane);
-        if (128 + 4 * lane < dp) po[u][1] = *reinterpret_cast<const float4*>(o + 128 + 4 * lane);
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) at += wcount[w];
+        found[k] += wcount[w];
       }
-    }
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
-    const float base = mn == -INFINITY ? 0.0f : mn, corr = exp2f(m - base);
-    m = mn;
-    l *= corr;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) acc[k].x *= corr, acc[k].y *= corr, acc[k].z *= corr, acc[k].w *= corr;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float w = exp2f(pm[u] - base);
-      l = fmaf(w, pl[u], l);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        acc[k].x = fmaf(w, po[u][k].x, acc[k].x);
-        acc[k].y = fmaf(w, po[u][k].y, acc[k].y);
-        acc[k].z = fmaf(w, po[u][k].z, acc[k].z);
-        acc[k].w = fmaf(w, po[u][k].w, acc[k].w);
-      }
+      if (there) list[k][at + __popc(votes & ((1u << lane) - 1))] = (unsigned short)i;
+      __syncthreads();
     }
   }
-  const int rr = cut.r0 + r, token = plan_token(a.p, rr);
-  T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + token) * a.os + (int64_t)(cut.h * a.p.group + rr - token * a.p.group) * d;
-  bool bad = false;
-  if constexpr (R == 1) {
-    *reinterpret_cast<float4*>(&part[warp][4 * lane]) = acc[0];
-    *reinterpret_cast<float4*>(&part[warp][128 + 4 * lane]) = acc[1];
-    if (lane == 0) ms[warp] = m, ls[warp] = l;
-    __syncthreads();
-    float mm = ms[0];
+  const int tasks0 = found[0] * parts.of[0].groups, tasks = tasks0 + found[1] * parts.of[1].groups;
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const bool second = task >= tasks0;
+    const KvPart& pt = parts.of[second];
+    const int number = second ? task - tasks0 : task, br = pt.br;
+    const int cta = list[second][number / pt.groups];
+    const KvCut cut = reinterpret_cast<const KvCut*>(pt.ws)[cta];
+    const int pieces = cut.pieces, r = (number % pt.groups) * R + warp / SPLIT;
+    if (r >= cut.rows) continue;  // R == 1: the whole CTA; else the warp has nobody to meet
+    const size_t slot = plan_slot_floats(br, dp), step = 2 * slot;
+    // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
+    const float* first = pt.ws + plan_cut_floats(pt.ctas) + (size_t)cta * step + slot;
+    const float* rest = first + slot;
+    constexpr int U = R == 1 ? 4 : 2;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc[NV] = {};  // features 4 lane .. (and 128 + 4 lane ..)
+    for (int i0 = warp % SPLIT; i0 < pieces; i0 += SPLIT * U) {
+      float pm[U], pl[U];
+      float4 po[U][NV];
 #pragma unroll
-    for (int k = 1; k < WARPS; ++k) mm = fmaxf(mm, ms[k]);
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float sum = 0.0f, o = 0.0f;
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * SPLIT;
+        pm[u] = -INFINITY, pl[u] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) {
-      const float w = exp2f(ms[k] - base);
-      sum = fmaf(w, ls[k], sum);
-      o = fmaf(w, part[k][threadIdx.x], o);
-    }
-    if ((int)threadIdx.x < d) {
-      o = sum == 0.0f ? 0.0f : o / sum;
-      out[threadIdx.x] = kv_from<T>(o);
-      bad = !isfinite(o);
-    }
-    bad = __syncthreads_or(bad) && warp == 0;
-  } else {
+        for (int k = 0; k < NV; ++k) po[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < pieces) {
+          const float* s = i == 0 ? first : rest + (size_t)(i - 1) * step;
+          const float* o = s + plan_slot_o(br) + (size_t)r * dp;
+          pm[u] = s[r];
+          pl[u] = s[br + r];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float f[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+          for (int k = 0; k < NV; ++k)
+            if (128 * k + 4 * lane < dp) po[u][k] = *reinterpret_cast<const float4*>(o + 128 * k + 4 * lane);
+        }
+      }
+      float mn = m;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = 128 * k + 4 * lane + e;
-        if (x < d) {
-          const float o = l == 0.0f ? 0.0f : f[e] / l;
-          out[x] = kv_from<T>(o);
-          bad |= !isfinite(o);
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+      const float base = mn == -INFINITY ? 0.0f : mn, corr = exp2f(m - base);
+      m = mn;
+      l *= corr;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) acc[k].x *= corr, acc[k].y *= corr, acc[k].z *= corr, acc[k].w *= corr;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = exp2f(pm[u] - base);
+        l = fmaf(w, pl[u], l);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          acc[k].x = fmaf(w, po[u][k].x, acc[k].x);
+          acc[k].y = fmaf(w, po[u][k].y, acc[k].y);
+          acc[k].z = fmaf(w, po[u][k].z, acc[k].z);
+          acc[k].w = fmaf(w, po[u][k].w, acc[k].w);
         }
       }
     }
-    bad = __any_sync(0xffffffffu, bad);
-  }
-  // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
-  if (bad) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
-  if constexpr (R == 1) __syncthreads();
+    const int rr = cut.r0 + r, token = plan_token(a.p, rr);
+    T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + token) * a.os + (int64_t)(cut.h * a.p.group + rr - token * a.p.group) * d;
+    bool bad = false;
+    if constexpr (R == 1) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) *reinterpret_cast<float4*>(&part[warp][128 * k + 4 * lane]) = acc[k];
+      if (lane == 0) ms[warp] = m, ls[warp] = l;
+      __syncthreads();
+      float mm = ms[0];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) mm = fmaxf(mm, ms[k]);
+      const float base = mm == -INFINITY ? 0.0f : mm;
+      if ((int)threadIdx.x < d) {
+        float sum = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) {
+          const float w = exp2f(ms[k] - base);
+          sum = fmaf(w, ls[k], sum);
+          o = fmaf(w, part[k][threadIdx.x], o);
+        }
+        o = sum == 0.0f ? 0.0f : o / sum;
+        out[threadIdx.x] = kv_from<T>(o);
+        bad = !isfinite(o);
+      }
+      bad = __syncthreads_or(bad) && warp == 0;
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const float f[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 128 * k + 4 * lane + e;
+          if (x < d) {
+            const float o = l == 0.0f ? 0.0f : f[e] / l;
+            out[x] = kv_from<T>(o);
+            bad |= !isfinite(o);
+          }
+        }
+      }
+      bad = __any_sync(0xffffffffu, bad);
+    }
+    // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
+    if (bad) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
+    if constexpr (R == 1) __syncthreads();
   }
 }
 
@@ -250,10 +271,14 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
   return count;
 }
 
+// Each launch has a part of the workspace (16-byte aligned: slots are).
+static size_t part_floats(const KvLaunch& l) {
+  return plan_cut_floats(l.ctas) + (size_t)l.ctas * 2 * plan_slot_floats(l.br, l.dp);
+}
 static size_t workspace_floats(const KvLaunch* l, int count) {
-  size_t most = 0;
-  for (int i = 0; i < count; ++i) most = std::max(most, plan_cut_floats(l[i].ctas) + (size_t)l[i].ctas * 2 * plan_slot_floats(l[i].br, l[i].dp));
-  return most;
+  size_t sum = 0;
+  for (int i = 0; i < count; ++i) sum += part_floats(l[i]);
+  return sum;
 }
 
 template <typename T>
@@ -262,10 +287,13 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
   const int count = pick<T>(a.c, a.bt.total, a.bt.n, q_heads, one_each, a.qvec, l);
   OC_REQUIRE(ws && aligned16(ws) && ws_bytes >= workspace_floats(l, count) * sizeof(float),
              "kv_attention: workspace too small or not 16-byte aligned");
+  KvParts parts = {};
+  a.ws = static_cast<float*>(ws);
+  int dp = 0, rows = 0;
   for (int i = 0; i < count; ++i) {
     a.p.br = l[i].br, a.p.bk_shift = __builtin_ctz(l[i].bk), a.p.rows_min = l[i].rows_min, a.p.rows_max = l[i].rows_max;
     a.p.ctas = l[i].ctas, a.p.min_units = l[i].min_units;
-    a.ws = static_cast<float*>(ws);
+    a.beside = i > 0;
     if (!smem_attr_once(l[i].fn(), l[i].smem)) return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
     const dim3 grid(l[i].ctas), block(l[i].threads);
     if (l[i].kern) {
@@ -273,12 +301,12 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
     } else {
       // the pools as matrices of head_dim columns; a box is a page, or a tile of a larger one
       const KvView& c = a.c;
-      const uint64_t rows = ((uint64_t)c.layers * c.pages * c.hk) << c.ps_shift;
-      const int box = c.ps_shift < 3 || rows > INT_MAX ? 0 : std::min(1 << c.ps_shift, l[i].bk);
+      const uint64_t pool_rows = ((uint64_t)c.layers * c.pages * c.hk) << c.ps_shift;
+      const int box = c.ps_shift < 3 || pool_rows > INT_MAX ? 0 : std::min(1 << c.ps_shift, l[i].bk);
       const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
       CUtensorMap m[3] = {};
       for (int x = 0; box && x < 2; ++x)
-        if (int rc = make_tmap_2d(&m[x], x ? c.v : c.k, type, sizeof(T), c.d, rows, (uint64_t)c.d * sizeof(T), 64, box,
+        if (int rc = make_tmap_2d(&m[x], x ? c.v : c.k, type, sizeof(T), c.d, pool_rows, (uint64_t)c.d * sizeof(T), 64, box,
                                   CU_TENSOR_MAP_SWIZZLE_128B))
           return rc;
       // the queries as [token][head][feature]: a box is all heads of a group, of 128 / G tokens
@@ -289,16 +317,27 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
           return rc;
       OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], m[2], box, qbox));
     }
-    if (l[i].ctas > 1)
-{
-      const bool few = l[i].merge_rows <= 16;
-      const int groups = few ? l[i].merge_rows : (l[i].merge_rows + 7) / 8;
-      const int64_t tasks = (int64_t)(l[i].ctas - 1) * groups;
-      const int grid = (int)std::min<int64_t>(tasks, 4 * (int64_t)std::max(1, sm_count()));
-      OC_CHECK_CUDA(launch_pdl_ex(few ? kv_merge_kernel<T, 1> : kv_merge_kernel<T, 8>, dim3(grid), dim3(256), 0, s, a, l[i].dp, groups));
-    }
+    parts.of[i] = KvPart{a.ws, l[i].ctas, l[i].br, 0};
+    a.ws += part_floats(l[i]);
+    dp = l[i].dp;
+    rows = std::max(rows, l[i].merge_rows);
   }
-  return OC_OK;
+  // the rows of one item that the joining kernel takes at a time: see there
+  const bool few = count == 1 && rows <= 16;
+  int64_t tasks = 0;
+  parts.count = count;
+  for (int i = 0; i < count; ++i) {
+    parts.of[i].groups = few ? l[i].merge_rows : (l[i].merge_rows + 7) / 8;
+    tasks += (int64_t)(l[i].ctas - 1) * parts.of[i].groups;
+  }
+  if (tasks == 0) return OC_OK;  // one CTA: nothing is cut
+  const int grid = (int)std::min<int64_t>(tasks, (few ? 4 : 8) * (int64_t)std::max(1, sm_count()));
+  auto go = [&](auto kern) {
+    OC_CHECK_CUDA(launch_pdl_ex(kern, dim3(grid), dim3(256), 0, s, a, parts, dp));
+    return OC_OK;
+  };
+  if (dp <= 128) return few ? go(kv_merge_kernel<T, 1, 128>) : go(kv_merge_kernel<T, 8, 128>);
+  return few ? go(kv_merge_kernel<T, 1, 256>) : go(kv_merge_kernel<T, 8, 256>);
 }
 
 static int attn_args(const oc_kv_cache* cache, KvView* c, int tokens, int n, int q_heads) {

@@ -228,6 +228,7 @@ struct KvAttn {
   int qvec;      // rows of q are
   int ovec16;    // rows of out are whole 16-byte chunks
   int ovec;      // pairs of elements of out are 4-byte aligned
+  int beside;    // follows a launch of the same call, and may run beside it
   float* ws;
   int* dev_status;
 };

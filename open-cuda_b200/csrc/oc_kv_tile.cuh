@@ -192,14 +192,21 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
   uint8_t* sk = base + 2 * K::TILE;
   uint8_t* sq = base + 4 * K::TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
+  // Behind the warp-level kernel of the same call there is nothing to wait for:
+  // that one lets this one start after its own wait, so all that came before
+  // is there, and the two write different rows.  The wait then comes last, so
+  // that this grid's end is the end of both.
+  if (!a.beside) pdl_wait();
   pdl_launch();
   const KvView& c = a.c;
   KvCursor cur;
   int64_t chunk;
   const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, cur);
   if (threadIdx.x == 0) plan_no_cut(a);
-  if (total == 0) return;
+  if (total == 0) {
+    pdl_wait();
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_empty, 1);
@@ -537,6 +544,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
     tc_fence_after();
     tmem_dealloc(tmem, K::TMEM_COLS);
   }
+  pdl_wait();
 }
 
 }  // namespace oc
