@@ -3,7 +3,7 @@
 #include <map>
 
 #include "oc_kv_plan.cuh"
-#include "oc_kv_tile.cuh"
+#include "oc_kv_tile32.cuh"
 
 namespace oc {
 
@@ -241,27 +241,30 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
   const int group = q_heads / c.hk;
   const int most = one_each ? group : tokens * group;                 // rows that a sequence can have
   const int likely = tokens <= n ? std::min(group, most) : most;      // and those to choose a shape by
-  int count = 1;
-  if (sizeof(T) == 2 && vector_rows(c, sizeof(T))) {
-    const bool tile = (c.d == 64 || c.d == 128) && qvec && tokens > n && most > kFewRows && is_sm100();
-    if constexpr (sizeof(T) == 2) {
-      out[0] = mma_launch<T>(c.d, tile ? kFewRows : likely);
-      if (tile) {
-        out[0].rows_max = kFewRows;
-        auto go = [](auto k) {
-          KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
-          l.tile = kv_tile_kernel<decltype(k)>;
-          return l;
-        };
-        out[1] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
-        out[1].rows_min = kFewRows;
-        out[1].one_per_sm = true;
-        count = 2;
-      }
+  const bool tile = (c.d == 64 || c.d == 128) && tokens > n && most > kFewRows && is_sm100() &&
+                    (sizeof(T) == 4 || (qvec && vector_rows(c, sizeof(T))));
+  if constexpr (sizeof(T) == 4) {
+    out[0] = scalar_launch<T>(c.d, tile ? kFewRows : likely);
+    if (tile) {
+      auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>, 2); };
+      out[1] = c.d == 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
     }
   } else {
-    out[0] = scalar_launch<T>(c.d, likely);
+    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, tile ? kFewRows : likely) : scalar_launch<T>(c.d, likely);
+    if (tile) {
+      auto go = [](auto k) {
+        KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
+        l.tile = kv_tile_kernel<decltype(k)>;
+        return l;
+      };
+      out[1] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
+    }
   }
+  if (tile) {
+    out[0].rows_max = out[1].rows_min = kFewRows;
+    out[1].one_per_sm = true;
+  }
+  const int count = tile ? 2 : 1;
   for (int i = 0; i < count; ++i) {
     const void* fn = out[i].fn();
     smem_attr_once(fn, out[i].smem);  // before the occupancy is asked for

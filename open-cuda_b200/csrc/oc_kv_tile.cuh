@@ -78,10 +78,11 @@ __device__ __forceinline__ float kv_max3(float x, float y, float z) {
   return r;
 }
 
-// A consumer's place in the ring of jobs.
+// A consumer's place in the ring of jobs; B has the barriers.
+template <typename B>
 struct KvJobs {
   const KvJob* ring;
-  KvTileBars* bar;
+  B* bar;
   uint32_t at = 0, phase = 0;
   // The next job; false when a wait gave up.  Whole warps, or one thread.
   template <bool WARP>
@@ -99,6 +100,19 @@ struct KvJobs {
   }
 };
 
+// The walking warp: hands out the piece at `cur` (none when nothing is left)
+// and notes the cut behind the run.  Returns where the piece ends.
+__device__ __forceinline__ int kv_hand_out(const KvAttn& a, const KvCursor& cur, int64_t left, int64_t chunk, KvJob* slot,
+                                           uint64_t* full) {
+  const int t0 = cur.at, t1 = left > 0 ? (int)min((int64_t)cur.it.units, t0 + left) : t0;
+  if ((threadIdx.x & 31) == 0) {
+    *slot = KvJob{cur.s, cur.b, cur.h, cur.it.r0, cur.it.rows, cur.it.lo, cur.it.hi, cur.it.tile0, cur.it.units, t0, t1};
+    if (t0 == 0 && t0 < t1 && t1 < cur.it.units) plan_cut(a, cur, cur.it.units - t1, chunk);
+    mbar_arrive(full);
+  }
+  return t1;
+}
+
 // 16-byte chunks of a 128-row tile: D / 8 lanes take a row, so a warp copies
 // RPI rows an instruction.
 template <typename K>
@@ -112,7 +126,7 @@ struct KvTileRows {
 // One warp: the K or the V tiles of a run.  `box`: keys a TMA box holds, 0
 // for pages that are too small.
 template <typename K>
-__device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs jobs, const CUtensorMap* map, const typename K::T* pool,
+__device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs<KvTileBars> jobs, const CUtensorMap* map, const typename K::T* pool,
                                              uint8_t* tiles, uint64_t* full, uint64_t* empty, int box, volatile int* abort_flag) {
   using T = typename K::T;
   using R = KvTileRows<K>;
@@ -236,7 +250,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  KvJobs jobs{ring, &bar};
+  KvJobs<KvTileBars> jobs{ring, &bar};
 
   if (warp == 0) {
     if (lane == 0) {
@@ -328,12 +342,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
       const uint32_t at = items % kJobs, ph = (items / kJobs) & 1;
       ok = warp_wait(&bar.job_empty[at], ph ^ 1, abort_flag);
       if (!ok) break;
-      const int t0 = cur.at, t1 = left > 0 ? (int)min((int64_t)cur.it.units, t0 + left) : t0;
-      if (lane == 0) {
-        ring[at] = KvJob{cur.s, cur.b, cur.h, cur.it.r0, cur.it.rows, cur.it.lo, cur.it.hi, cur.it.tile0, cur.it.units, t0, t1};
-        if (t0 == 0 && t0 < t1 && t1 < cur.it.units) plan_cut(a, cur, cur.it.units - t1, chunk);
-        mbar_arrive(&bar.job_full[at]);
-      }
+      const int t0 = cur.at, t1 = kv_hand_out(a, cur, left, chunk, &ring[at], &bar.job_full[at]);
       if (t0 == t1) break;
       ok = warp_wait(&bar.q_empty, (items & 1) ^ 1, abort_flag);
       if (!ok) break;

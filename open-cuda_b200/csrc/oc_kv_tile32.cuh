@@ -1,0 +1,473 @@
+// oc_kv_tile32.cuh -- attention over the paged cache for chunks of new tokens
+// in f32, head_dim 64 and 128, on the tcgen05 tensor cores.
+//
+// The arithmetic is flash_tc_kernel's (oc_flash_tc.cuh): every operand as two
+// f16 terms of a power-of-two scaling (Q and K per row, V per tile, P by
+// 2^15), three MMAs per product step, scores in log2 units, the running output
+// rescaled with every tile.  What differs is where rows come from and how the
+// work is shared out: query rows are the heads of a kv head of consecutive
+// tokens, key rows are looked up page by page (zeros where no row of the item
+// sees a key), a CTA works through a run of pieces (oc_kv_plan.cuh), and what
+// a cut leaves goes to the workspace.
+//
+// Bound: the conversion of K and V (each element once per item: two f16 terms
+// take about ten instructions a pair) and the chain S -> softmax -> P V of a
+// tile, not the tensor pipe; 8 prompts of 300 to 777 tokens over 12 heads of
+// 64 measured: see the table of the operators.
+//
+// One CTA an SM, 448 threads:
+//   warp 0       TMEM allocator + MMA issuer (lane 0)
+//   warps 1..8   converters: f32 rows -> f16 terms in swizzled tiles
+//   warps 9..12  softmax and output: thread = query row = TMEM lane
+//   warp 13      walks the CTA's run and hands its pieces to the others
+#pragma once
+#include "oc_kv_tile.cuh"
+
+namespace oc {
+
+template <int D_>
+struct KvTile32 {
+  static constexpr int D = D_, DP = D_, ROWS = 128, BK = 128, THREADS = 32 * 14;
+  static constexpr int PANEL = 128 * 128, TILE = 128 * D * 2;  // bytes: 64 features, one term of 128 rows
+  static constexpr int S_COL = 0, O_COL = 128, A_COL = 128 + D, TMEM_COLS = D == 64 ? 256 : 512;
+  static constexpr size_t SMEM = 1024 + 6 * (size_t)TILE;
+};
+
+struct KvTile32Shared {
+  uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, o_empty, vmax;
+  uint64_t job_full[kJobs], job_empty[kJobs];
+  KvJob ring[kJobs];
+  float icq[2][128];       // 1 / c_q per query row, by the piece's parity
+  float ick[2][128];       // 1 / c_k per key row, with the sign of the scale, by the tile's parity
+  float icv[2];            // 1 / c_v of the V tile
+  float vpart[2][kFaConv]; // converter warps' max |v|
+  uint32_t rough[2];       // by the piece's parity: its number + 1 when V's rows are too uneven for its masks
+  uint32_t tmem;
+  int abort_word;
+};
+
+// The converter warp's 16 rows of a 128-row tile, from the offsets that its
+// lanes 0..15 hold (-1: a row of zeros): fa_convert_tile with rows anywhere.
+// `rough` (TILE, when given): set to `id` when one row is so much larger than
+// another that the common scaling leaves the smaller too few bits.  Rows that
+// see both do not mind; one that sees the smaller alone does, so this is
+// asked of tiles that some row sees in part.
+template <int D, bool TILE>
+__device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, int64_t off, bool vec, uint8_t* thi,
+                                                uint8_t* tlo, float* inv, float sign, int w, int lane, float* part,
+                                                uint64_t* vmax, uint32_t ph, volatile int* abort_flag,
+                                                uint32_t* rough = nullptr, uint32_t id = 0) {
+  constexpr int RPW = 128 / kFaConv, LPR = D / 4, RPS = 32 / LPR, NS = RPW / RPS;
+  const int q4 = lane % LPR, ro = lane / LPR;
+  float4 x[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int64_t o = __shfl_sync(0xffffffffu, off, s * RPS + ro);
+    x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (o >= 0) {
+      const float* p = base + o + 4 * q4;
+      if (vec)
+        x[s] = *reinterpret_cast<const float4*>(p);
+      else
+        x[s] = make_float4(p[0], p[1], p[2], p[3]);
+    }
+  }
+  float cr[NS];
+  if constexpr (TILE) {
+    float mx = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) mx = fmaxf(mx, fa_absmax4(x[s]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) {
+      part[w] = mx;
+      mbar_arrive(vmax);
+    }
+    if (!warp_wait(vmax, ph, abort_flag)) return false;
+    float m = part[0];
+#pragma unroll
+    for (int j = 1; j < kFaConv; ++j) m = fmaxf(m, part[j]);
+    const int ce = fa_range_exp(m);
+    if (rough) {
+      bool uneven = false;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        float rm = fa_absmax4(x[s]);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) rm = fmaxf(rm, __shfl_xor_sync(0xffffffffu, rm, o));
+        uneven |= rm > 0.0f && rm < m * 0.00390625f;
+      }
+      if (__any_sync(0xffffffffu, uneven) && lane == 0) *reinterpret_cast<volatile uint32_t*>(rough) = id;
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) cr[s] = exp2_int(ce);
+    if (w == 0 && lane == 0) *inv = exp2_int(-ce);
+  } else {
+    float mx[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) mx[s] = fa_absmax4(x[s]);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) mx[s] = fmaxf(mx[s], __shfl_xor_sync(0xffffffffu, mx[s], o));
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int ce = fa_range_exp(mx[s]);
+      if (q4 == 0) inv[w * RPW + s * RPS + ro] = __fmul_rn(sign, exp2_int(-ce));
+      cr[s] = exp2_int(ce);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    uint2 hi, lo;
+    fa_split4(x[s], cr[s], hi, lo);
+    const uint32_t to = fa_tile_off(w * RPW + s * RPS + ro, 4 * q4);
+    *reinterpret_cast<uint2*>(thi + to) = hi;
+    *reinterpret_cast<uint2*>(tlo + to) = lo;
+  }
+  return true;
+}
+
+// fa_max_chunk and fa_p_chunk for a row that sees keys [from, to) of the chunk.
+__device__ __forceinline__ float kv_max_chunk(const uint32_t (&r)[32], const float* ik, int from, int to, float tmax) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j >= from && j < to) tmax = fmaxf(tmax, __fmul_rn(__uint_as_float(r[j]), ik[j]));
+  return tmax;
+}
+__device__ __forceinline__ float kv_p_chunk(const uint32_t (&r)[32], const float* ik, float rq2, float nb, int from, int to,
+                                            uint32_t (&ph16)[16], uint32_t (&pl16)[16]) {
+  float psum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float p[2], h[2], l[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float x = __fmaf_rn(__fmul_rn(__uint_as_float(r[j + u]), ik[j + u]), rq2, nb);
+      // (a NaN goes through: fminf would drop it)
+      p[u] = j + u >= from && j + u < to ? fa_ex2(x > 15.0f ? 15.0f : x) : 0.0f;
+      psum = __fadd_rn(psum, p[u]);
+      fa_split(p[u], h[u], l[u]);
+    }
+    ph16[j >> 1] = fa_pack_f16x2(h[0], h[1]);
+    pl16[j >> 1] = fa_pack_f16x2(l[0], l[1]);
+  }
+  return psum;
+}
+
+template <typename K>
+__global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
+  constexpr int D = K::D;
+  extern __shared__ uint8_t raw[];
+  __shared__ KvPlanShared plan;
+  __shared__ KvTile32Shared sh;
+  volatile int* abort_flag = &sh.abort_word;
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  // V precedes K: the V descriptors' reach stays inside the allocation
+  uint8_t *q_hi = base, *q_lo = q_hi + K::TILE, *v_hi = q_lo + K::TILE, *v_lo = v_hi + K::TILE, *k_hi = v_lo + K::TILE,
+          *k_lo = k_hi + K::TILE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (!a.beside) pdl_wait();  // (oc_kv_tile.cuh)
+  pdl_launch();
+  const KvView& c = a.c;
+  KvCursor cur;
+  int64_t chunk;
+  const int64_t total = plan_locate(a.p, c, a.bt, blockIdx.x, &plan, &chunk, cur);
+  if (threadIdx.x == 0) plan_no_cut(a);
+  if (total == 0) {
+    pdl_wait();
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, kFaConv);
+    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.k_full, kFaConv);
+    mbar_init(&sh.k_empty, 1);
+    mbar_init(&sh.v_full, kFaConv);
+    mbar_init(&sh.v_empty, 1);
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.p_full, 4);
+    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.o_empty, 4);
+    mbar_init(&sh.vmax, kFaConv);
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(&sh.job_full[i], 1);
+      mbar_init(&sh.job_empty[i], 1 + kFaConv + 4);
+    }
+    sh.abort_word = 0;
+    sh.rough[0] = sh.rough[1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&sh.tmem, K::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  KvJobs<KvTile32Shared> jobs{sh.ring, &sh};
+
+  if (warp == 0) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = idesc_f16(128, 128);
+      constexpr uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // B (V) MN-major
+      bool ok = true;
+      uint32_t n = 0, items = 0;
+      for (;;) {
+        KvJob it;
+        ok = jobs.template take<false>(it, abort_flag);
+        const int tiles = it.t1 - it.t0;
+        if (!ok || tiles == 0) break;
+        ok = mbar_wait(&sh.q_full, items & 1, abort_flag);
+        for (int t = 0; ok && t < tiles; ++t, ++n) {
+          const uint32_t ph = n & 1u;
+          ok = mbar_wait(&sh.k_full, ph, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          // S' = Q' K'^T: per 16-feature step, hi.hi + hi.lo + lo.hi
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk >> 2) * K::PANEL + (uint32_t)(kk & 3) * 32;
+            const uint64_t qh = desc_kmajor_sw128(smem_u32(q_hi) + off), ql = desc_kmajor_sw128(smem_u32(q_lo) + off);
+            const uint64_t kh = desc_kmajor_sw128(smem_u32(k_hi) + off), kl = desc_kmajor_sw128(smem_u32(k_lo) + off);
+            mma_f16(tmem + K::S_COL, qh, kh, idesc_s, kk != 0 ? 1u : 0u);
+            mma_f16(tmem + K::S_COL, qh, kl, idesc_s, 1u);
+            mma_f16(tmem + K::S_COL, ql, kh, idesc_s, 1u);
+          }
+          tc_commit(&sh.s_full);
+          tc_commit(&sh.k_empty);
+          if (t + 1 == tiles) tc_commit(&sh.q_empty);
+          // O' = P' V': wait for P, V, and for the previous O' to be read
+          ok = mbar_wait(&sh.p_full, ph, abort_flag) && mbar_wait(&sh.v_full, ph, abort_flag) &&
+               mbar_wait(&sh.o_empty, ph ^ 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < K::BK / 16; ++kk) {
+            const uint32_t off = (uint32_t)kk * 2048;
+            const uint64_t vh = desc_mnmajor_sw128(smem_u32(v_hi) + off, K::PANEL, 1024);
+            const uint64_t vl = desc_mnmajor_sw128(smem_u32(v_lo) + off, K::PANEL, 1024);
+            // P of keys [16 kk, 16 kk + 16): chunk kk / 2 of S's columns, hi in its first 16 columns, lo in the next 16
+            const uint32_t pcol = tmem + K::S_COL + (uint32_t)(kk >> 1) * 32 + (uint32_t)(kk & 1) * 8;
+            mma_f16_ta(tmem + K::O_COL, pcol, vh, idesc_o, kk != 0 ? 1u : 0u);
+            mma_f16_ta(tmem + K::O_COL, pcol, vl, idesc_o, 1u);
+            mma_f16_ta(tmem + K::O_COL, pcol + 16, vh, idesc_o, 1u);
+          }
+          tc_commit(&sh.o_full);
+          tc_commit(&sh.v_empty);
+        }
+        if (!ok) break;
+        ++items;
+        jobs.template drop<false>();
+      }
+      if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutMma);
+    }
+  } else if (warp <= kFaConv) {
+    const int w = warp - 1, mine = w * 16 + (lane & 15);  // row whose offset this lane looks up
+    const float ksign = a.scale2 < 0.0f ? -1.0f : 1.0f;
+    const float* kb = static_cast<const float*>(c.k) + a.layer_off;
+    const float* vb = static_cast<const float*>(c.v) + a.layer_off;
+    bool ok = true;
+    uint32_t n = 0, items = 0;
+    for (;;) {
+      KvJob it;
+      ok = jobs.template take<true>(it, abort_flag);
+      if (!ok || it.t0 == it.t1) break;
+      ok = warp_wait(&sh.q_empty, (items & 1) ^ 1, abort_flag);
+      if (!ok) break;
+      const int rr = it.r0 + mine, token = plan_token(a.p, rr);
+      const int64_t qoff = mine < it.rows ? (int64_t)(it.s.q0 + token) * a.qs + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D : -1;
+      kv_convert_tile<D, false>(static_cast<const float*>(a.q), qoff, a.qvec, q_hi, q_lo, sh.icq[items & 1], 1.0f, w, lane, nullptr, nullptr, 0,
+                                abort_flag);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+      // keys that all rows of the item see
+      int all_lo, all_hi, unused;
+      plan_row_range(a.p, it.s, it.r0, unused, all_hi);
+      plan_row_range(a.p, it.s, it.r0 + it.rows - 1, all_lo, unused);
+      int64_t next = kv_row_off(a, it.s.s, it.h, (it.tile0 + it.t0) * K::BK + mine, it.lo, it.hi);
+      for (int t = it.t0; t < it.t1; ++t, ++n) {
+        const uint32_t ph = n & 1u;
+        const int64_t off = next;
+        if (t + 1 < it.t1) next = kv_row_off(a, it.s.s, it.h, (it.tile0 + t + 1) * K::BK + mine, it.lo, it.hi);
+        ok = warp_wait(&sh.k_empty, ph ^ 1u, abort_flag);
+        if (!ok) break;
+        kv_convert_tile<D, false>(kb, off, a.vec, k_hi, k_lo, sh.ick[ph], ksign, w, lane, nullptr, nullptr, 0, abort_flag);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.k_full);
+        const int first = max((it.tile0 + t) * K::BK, it.lo), last = min((it.tile0 + t + 1) * K::BK, it.hi);
+        const bool masked = first < all_lo || last > all_hi;  // (zeros stand in place of keys that no row sees)
+        ok = warp_wait(&sh.v_empty, ph ^ 1u, abort_flag) &&
+             kv_convert_tile<D, true>(vb, off, a.vec, v_hi, v_lo, &sh.icv[ph], 1.0f, w, lane, sh.vpart[ph], &sh.vmax, ph, abort_flag,
+                                      masked ? &sh.rough[items & 1] : nullptr, items + 1);
+        if (!ok) break;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.v_full);
+      }
+      if (!ok) break;
+      ++items;
+      jobs.template drop<true>();
+    }
+    if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
+  } else if (warp <= kFaConv + 4) {
+    const int quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    bool ok = true;
+    uint32_t n = 0, items = 0;
+    for (;;) {
+      KvJob it;
+      ok = jobs.template take<true>(it, abort_flag);
+      const int t0 = it.t0, t1 = it.t1;
+      if (!ok || t0 == t1) break;
+      int lo = 0, hi = 0;
+      if (row < it.rows) plan_row_range(a.p, it.s, it.r0 + row, lo, hi);
+      float rq2 = 0.0f;
+      float m_i = -INFINITY, l_i = 0.0f;  // running max (log2 units) and 2^15-scaled sum
+      for (int t = t0; t < t1; ++t, ++n) {
+        const uint32_t ph = n & 1u;
+        const int key0 = (it.tile0 + t) * K::BK, from = lo - key0, to = hi - key0;  // keys of this tile that are seen
+        const bool all = from <= 0 && to >= K::BK;
+        const float* ik = sh.ick[ph];
+        ok = warp_wait(&sh.s_full, ph, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        // |scale| * log2(e) / c_q; the sign of scale rides on the key factors.
+        // (S was computed from the queries, so their factors are there too; the
+        // barrier of the queries may be phases ahead of this warp by now.)
+        if (t == t0) rq2 = __fmul_rn(fabsf(a.scale2), sh.icq[items & 1][row]);
+        // pass 1: the tile's max of S' * sign / c_k (rq2 >= 0 keeps the order)
+        float tmax = -INFINITY;
+#pragma unroll 1
+        for (int cb = 0; cb < 4; ++cb) {
+          uint32_t r[32];
+          tmem_ld32(lanes + K::S_COL + cb * 32, r);
+          tmem_ld_wait();
+          tmax = all ? fa_max_chunk<false>(r, ik + cb * 32, 32, tmax) : kv_max_chunk(r, ik + cb * 32, from - cb * 32, to - cb * 32, tmax);
+        }
+        const float tm = tmax == -INFINITY ? -INFINITY : __fmul_rn(tmax, rq2);
+        const float new_m = fmaxf(m_i, tm);
+        const float corr = (m_i == -INFINITY) ? 0.0f : fa_ex2(__fsub_rn(m_i, new_m));
+        // pass 2: p, the tile's sum, P terms into tensor memory.  Past |m'| =
+        // 2^20 the rounding of 15 - m' can reach an exponent above 15, so that
+        // range (and partly visible tiles) takes the guarded path.
+        const bool dead = new_m == -INFINITY;
+        const bool guard = dead || !all || fabsf(new_m) > 1048576.0f;
+        const float nb = dead ? 0.0f : __fsub_rn(15.0f, new_m);
+        const int f2 = dead ? 0 : from, e2 = dead ? 0 : to;
+        float psum = 0.0f;
+#pragma unroll 1
+        for (int cb = 0; cb < 4; ++cb) {
+          uint32_t r[32];
+          tmem_ld32(lanes + K::S_COL + cb * 32, r);
+          tmem_ld_wait();
+          uint32_t ph16[16], pl16[16];
+          psum = __fadd_rn(psum, guard ? kv_p_chunk(r, ik + cb * 32, rq2, nb, f2 - cb * 32, e2 - cb * 32, ph16, pl16)
+                                       : fa_p_chunk<false>(r, ik + cb * 32, rq2, nb, 32, ph16, pl16));
+          // over S' chunk cb, which this thread has read
+          tmem_st16(lanes + K::S_COL + cb * 32, ph16);
+          tmem_st16(lanes + K::S_COL + cb * 32 + 16, pl16);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full);
+        l_i = __fmaf_rn(l_i, corr, psum);
+        m_i = new_m;
+        // O' of this tile -> o = o * corr + O' / c_v
+        ok = warp_wait(&sh.o_full, ph, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const float iv = sh.icv[ph];
+#pragma unroll 1
+        for (int cb = 0; cb < D / 32; ++cb) {
+          uint32_t r[32], o[32];
+          tmem_ld32(lanes + K::O_COL + cb * 32, r);
+          if (t > t0) tmem_ld32(lanes + K::A_COL + cb * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int f = 0; f < 32; ++f)
+            o[f] = __float_as_uint(
+                __fmaf_rn(__uint_as_float(r[f]), iv, t > t0 ? __fmul_rn(__uint_as_float(o[f]), corr) : 0.0f));
+          tmem_st32(lanes + K::A_COL + cb * 32, o);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.o_empty);
+      }
+      if (!ok) break;
+      const bool whole = t0 == 0 && t1 == it.units, rough = *reinterpret_cast<volatile uint32_t*>(&sh.rough[items & 1]) == items + 1;
+      const int rr = it.r0 + row, token = plan_token(a.p, rr);
+      const float inv = l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
+      float* dst = whole ? static_cast<float*>(a.out) + (int64_t)(it.s.q0 + token) * a.os + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D
+                         : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D) + plan_slot_o(K::ROWS) + (size_t)row * D;
+      const bool vec = !whole || a.ovec16;
+      if (!whole && row < it.rows) {
+        float* slot = plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D);
+        slot[row] = m_i, slot[K::ROWS + row] = rough ? NAN : l_i;  // the merge computes such rows again
+      }
+      bool bad = whole && rough && row < it.rows;
+#pragma unroll 1
+      for (int cb = 0; cb < D / 32; ++cb) {
+        uint32_t o[32];
+        tmem_ld32(lanes + K::A_COL + cb * 32, o);
+        tmem_ld_wait();
+        if (row < it.rows) {
+#pragma unroll
+          for (int f = 0; f < 32; f += 4) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = __uint_as_float(o[f + e]);
+              if (whole) {
+                // the quotient with one rounding more than the division's
+                y[e] = __fmul_rn(y[e], inv);
+                bad |= !isfinite(y[e]);
+              }
+            }
+            if (vec) {
+              *reinterpret_cast<float4*>(dst + cb * 32 + f) = make_float4(y[0], y[1], y[2], y[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dst[cb * 32 + f + e] = y[e];
+            }
+          }
+        }
+      }
+      const uint32_t rows_bad = __ballot_sync(0xffffffffu, bad);
+      __syncwarp();
+      for (uint32_t todo = rows_bad; todo; todo &= todo - 1)
+        kv_row_exact<float>(a, it.s, it.h, it.r0 + quad * 32 + __ffs(todo) - 1);
+      tc_fence_before();  // the running output's columns belong to these warps alone
+      ++items;
+      jobs.template drop<true>();
+    }
+    if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutEpilogue);
+  } else {
+    int64_t left = min(chunk, total - chunk * blockIdx.x);
+    bool ok = true;
+    for (uint32_t items = 0;; ++items) {
+      const uint32_t at = items % kJobs, ph = (items / kJobs) & 1;
+      ok = warp_wait(&sh.job_empty[at], ph ^ 1, abort_flag);
+      if (!ok) break;
+      const int t0 = cur.at, t1 = kv_hand_out(a, cur, left, chunk, &sh.ring[at], &sh.job_full[at]);
+      if (t0 == t1) break;
+      left -= t1 - t0;
+      if (left > 0) plan_next(a.p, c, a.bt, cur);
+    }
+    if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, K::TMEM_COLS);
+  }
+  pdl_wait();
+}
+
+}  // namespace oc

@@ -189,8 +189,14 @@ class KVCache:
 
     def check(self):
         """Waits for the cache's device and raises ValueError if a call since
-        the last check met something it refuses."""
+        the last check met something it refuses, OcError if a wait inside a
+        kernel expired."""
         bits = int(self.status.item())
+        expired = oc.ci(0)
+        with self._torch.cuda.device(self._index):
+            oc.check(oc.lib().oc_get_device_status(C.byref(expired)))
+        if expired.value:
+            raise oc.OcError(oc.OC_ERR_TIMEOUT, f"kv_cache: a wait inside a kernel expired (code {expired.value})")
         if bits:
             self.status.zero_()
             raise ValueError("kv_cache: " + "; ".join(text for bit, text in _REASONS.items() if bits & bit))

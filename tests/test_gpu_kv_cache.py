@@ -170,7 +170,7 @@ def test_fewer_tokens_than_sequences(dtype, d):
     check(dtype, 8, 2, d, 32, [9000, 40], [9, 1], seed=d)
 
 
-@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq, hk", [(1, 1), (7, 1), (8, 2), (9, 3), (40, 1)])
 def test_tiles_of_every_shape(dtype, d, hq, hk):
@@ -256,6 +256,24 @@ def test_what_a_row_does_not_see_has_no_part(dtype, d, what, new):
     close(o[:-1], want[:-1], tol[:-1])
     if math.isnan(what):
         assert torch.isnan(o[-1]).all()  # what a row does see counts
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new, n", [(9, 260), (200, 260), (200, 6000)])
+def test_f32_values_of_very_different_size(d, new, n):
+    """A value of 1e30 among values of 1e-10: the rows that do not see it, and
+    the ones that do."""
+    c, ks, vs = filled(F32, 2, d, 16, [n])
+    big = vs[0][:, n - 5] * 1e30
+    vs[0] = vs[0] * 1e-10
+    vs[0][:, n - 5] = big
+    for j in range(n):
+        page = int(c.page_table[0, j // 16])
+        c.v[0, page, :, j % 16] = vs[0][:, j]
+    q = torch.randn(new, 4, d, device="cuda")
+    o = attend(c, q, [0], [new])
+    want, tol = expected(q, ks, vs, [0], [new], 1 / math.sqrt(d), True, 0)
+    close(o, want, tol)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
