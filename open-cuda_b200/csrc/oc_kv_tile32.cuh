@@ -3,7 +3,7 @@
 //
 // The arithmetic is flash_tc_kernel's (oc_flash_tc.cuh): every operand as two
 // f16 terms of a power-of-two scaling (Q and K per row, V per tile, P by
-// 2^15), three MMAs per product step, scores in log2 units, the running output
+// 2^15), three MMAs per product step (the small terms first), scores in log2 units, the running output
 // rescaled with every tile.  What differs is where rows come from and how the
 // work is shared out: query rows are the heads of a kv head of consecutive
 // tokens, key rows are looked up page by page (zeros where no row of the item
@@ -225,16 +225,21 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
           ok = mbar_wait(&sh.k_full, ph, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          // S' = Q' K'^T: per 16-feature step, hi.hi + hi.lo + lo.hi
+          // S' = Q' K'^T: hi.lo and lo.hi of all features, then hi.hi.  Every
+          // addition to the accumulator is rounded at the size that the sum
+          // has by then (towards zero): the small terms first leave a third
+          // of the roundings at the full size.
+          auto terms = [&](const uint8_t* q, const uint8_t* k, uint32_t first) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (uint32_t)(kk >> 2) * K::PANEL + (uint32_t)(kk & 3) * 32;
-            const uint64_t qh = desc_kmajor_sw128(smem_u32(q_hi) + off), ql = desc_kmajor_sw128(smem_u32(q_lo) + off);
-            const uint64_t kh = desc_kmajor_sw128(smem_u32(k_hi) + off), kl = desc_kmajor_sw128(smem_u32(k_lo) + off);
-            mma_f16(tmem + K::S_COL, qh, kh, idesc_s, kk != 0 ? 1u : 0u);
-            mma_f16(tmem + K::S_COL, qh, kl, idesc_s, 1u);
-            mma_f16(tmem + K::S_COL, ql, kh, idesc_s, 1u);
-          }
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (uint32_t)(kk >> 2) * K::PANEL + (uint32_t)(kk & 3) * 32;
+              mma_f16(tmem + K::S_COL, desc_kmajor_sw128(smem_u32(q) + off), desc_kmajor_sw128(smem_u32(k) + off), idesc_s,
+                      first && kk == 0 ? 0u : 1u);
+            }
+          };
+          terms(q_hi, k_lo, 1u);
+          terms(q_lo, k_hi, 0u);
+          terms(q_hi, k_hi, 0u);
           tc_commit(&sh.s_full);
           tc_commit(&sh.k_empty);
           if (t + 1 == tiles) tc_commit(&sh.q_empty);
@@ -243,17 +248,16 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
                mbar_wait(&sh.o_empty, ph ^ 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
+          // P of keys [16 kk, 16 kk + 16): chunk kk / 2 of S's columns, hi in its first 16 columns, lo in the next 16
+          auto products = [&](uint32_t lo, const uint8_t* v, uint32_t first) {
 #pragma unroll
-          for (int kk = 0; kk < K::BK / 16; ++kk) {
-            const uint32_t off = (uint32_t)kk * 2048;
-            const uint64_t vh = desc_mnmajor_sw128(smem_u32(v_hi) + off, K::PANEL, 1024);
-            const uint64_t vl = desc_mnmajor_sw128(smem_u32(v_lo) + off, K::PANEL, 1024);
-            // P of keys [16 kk, 16 kk + 16): chunk kk / 2 of S's columns, hi in its first 16 columns, lo in the next 16
-            const uint32_t pcol = tmem + K::S_COL + (uint32_t)(kk >> 1) * 32 + (uint32_t)(kk & 1) * 8;
-            mma_f16_ta(tmem + K::O_COL, pcol, vh, idesc_o, kk != 0 ? 1u : 0u);
-            mma_f16_ta(tmem + K::O_COL, pcol, vl, idesc_o, 1u);
-            mma_f16_ta(tmem + K::O_COL, pcol + 16, vh, idesc_o, 1u);
-          }
+            for (int kk = 0; kk < K::BK / 16; ++kk)
+              mma_f16_ta(tmem + K::O_COL, tmem + K::S_COL + lo + (uint32_t)(kk >> 1) * 32 + (uint32_t)(kk & 1) * 8,
+                         desc_mnmajor_sw128(smem_u32(v) + (uint32_t)kk * 2048, K::PANEL, 1024), idesc_o, first && kk == 0 ? 0u : 1u);
+          };
+          products(0, v_lo, 1u);
+          products(16, v_hi, 0u);
+          products(0, v_hi, 0u);
           tc_commit(&sh.o_full);
           tc_commit(&sh.v_empty);
         }
