@@ -13,6 +13,7 @@
 
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "oc_internal.h"
 #include "oc_ptx.cuh"
@@ -70,6 +71,24 @@ template <>
 __device__ __forceinline__ __half kv_from<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 kv_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// {a, b} rounded to T and packed (a in the low half).
+template <typename T>
+__device__ __forceinline__ uint32_t kv_pack2(float a, float b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 kv_unpack2(uint32_t x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<__half2*>(&x));
+  else
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 
 // 16 bytes of T as floats and back.
 template <typename T>

@@ -6,10 +6,10 @@
 //   (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t),
 //   t = position * inv_freq[j]
 //
-// Nothing is computed twice that memory would wait for, so the bound is the
-// bytes: each element is read once and written once, 16 bytes a lane.  One
-// CTA works on one token (or, when there are few tokens, on a share of its
-// heads); its cosines and sines are computed once, in turns: t / (2 pi) in
+// Nothing is computed that memory would wait for, so the bound is the bytes:
+// each element is read once and written once, 16 bytes a lane.  Few tokens: a
+// CTA for a share of a token's heads; many: a warp a token.  The cosines and
+// sines are computed once a token, in turns: t / (2 pi) in
 // f64, reduced to [-1/2, 1/2] exactly before sincospif, so an angle of a far
 // position keeps f32 accuracy (f32 products lose 1e-2 at position 1e5).  A
 // lane holds eight features of a head that contain both members of its pairs
@@ -39,86 +39,77 @@ constexpr int kAppendThreads = 256;
 // past the rotated ones, and for interleaved pairs, eight consecutive ones.
 template <typename T, bool SPLIT>
 struct Octet {
-  static __device__ __forceinline__ bool paired(int u, int rot) { return !SPLIT || 8 * u < rot; }
-  static __device__ __forceinline__ void load(const T* x, int u, int rot, float (&f)[8]) {
-    if (SPLIT && 8 * u < rot) {
-      quad(x + 4 * u, f);
-      quad(x + rot / 2 + 4 * u, f + 4);
+  using Quad = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;  // four features
+  struct Raw {
+    Quad lo, hi;
+  };
+  static __device__ __forceinline__ void load(const T* x, int u, int rot, Raw& r) {
+    const bool pairs = SPLIT && 8 * u < rot;
+    r.lo = *reinterpret_cast<const Quad*>(x + (pairs ? 4 * u : 8 * u));
+    r.hi = *reinterpret_cast<const Quad*>(x + (pairs ? rot / 2 + 4 * u : 8 * u + 4));
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float (&f)[8]) {
+    if constexpr (sizeof(T) == 4) {
+      const float* p = reinterpret_cast<const float*>(&r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = p[i];
     } else {
-      quad(x + 8 * u, f);
-      quad(x + 8 * u + 4, f + 4);
+      const uint32_t p[4] = {r.lo.x, r.lo.y, r.hi.x, r.hi.y};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = kv_unpack2<T>(p[i]);
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+      }
     }
+  }
+  static __device__ __forceinline__ void norm(float (&f)[8], float inv, const Raw& weight) {
+    float w[8];
+    values(weight, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = f[e] * inv * w[e];
+  }
+  // Pair e of the four, by cosine and sine.
+  static __device__ __forceinline__ void turn(float (&f)[8], int e, float2 g) {
+    const int p = SPLIT ? e : 2 * e, q = SPLIT ? e + 4 : 2 * e + 1;
+    const float x = f[p], y = f[q];
+    f[p] = x * g.x - y * g.y;
+    f[q] = y * g.x + x * g.y;
+  }
+  static __device__ __forceinline__ void store(T* y, int u, int rot, const Raw& r) {
+    const bool pairs = SPLIT && 8 * u < rot;
+    *reinterpret_cast<Quad*>(y + (pairs ? 4 * u : 8 * u)) = r.lo;
+    *reinterpret_cast<Quad*>(y + (pairs ? rot / 2 + 4 * u : 8 * u + 4)) = r.hi;
   }
   static __device__ __forceinline__ void store(T* y, int u, int rot, const float (&f)[8]) {
-    if (SPLIT && 8 * u < rot) {
-      put(y + 4 * u, f);
-      put(y + rot / 2 + 4 * u, f + 4);
-    } else {
-      put(y + 8 * u, f);
-      put(y + 8 * u + 4, f + 4);
-    }
-  }
-  static __device__ __forceinline__ void quad(const T* x, float* f) {
+    Raw r;
     if constexpr (sizeof(T) == 4) {
-      const float4 r = *reinterpret_cast<const float4*>(x);
-      f[0] = r.x, f[1] = r.y, f[2] = r.z, f[3] = r.w;
+      r.lo = make_float4(f[0], f[1], f[2], f[3]);
+      r.hi = make_float4(f[4], f[5], f[6], f[7]);
     } else {
-      const uint2 r = *reinterpret_cast<const uint2*>(x);
-      const T* p = reinterpret_cast<const T*>(&r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = kv_f32(p[i]);
+      r.lo = make_uint2(kv_pack2<T>(f[0], f[1]), kv_pack2<T>(f[2], f[3]));
+      r.hi = make_uint2(kv_pack2<T>(f[4], f[5]), kv_pack2<T>(f[6], f[7]));
     }
-  }
-  static __device__ __forceinline__ void put(T* y, const float* f) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(y) = make_float4(f[0], f[1], f[2], f[3]);
-    } else {
-      uint2 r;
-      T* p = reinterpret_cast<T*>(&r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = kv_from<T>(f[i]);
-      *reinterpret_cast<uint2*>(y) = r;
-    }
+    store(y, u, rot, r);
   }
 };
 
-// Where the token of this CTA belongs; filled by kv_find_token.
-struct KvToken {
-  int pos;   // position in the sequence, negative when it holds fewer tokens than are new
-  int seq;   // row of the page table
-  bool ok;
-};
-
-// All threads: the entry whose new tokens contain token t.  An entry whose
-// sequence stands earlier in the list as well is refused (two entries would
-// write the same places).
-__device__ __forceinline__ KvToken kv_find_token(const KvView& c, const KvBatch& bt, int t, int* slot) {
-  KvToken r{0, -1, false};
-  if (threadIdx.x == 0) *slot = -1;
-  __syncthreads();
-  if (bt.cu) {
-    for (int b = threadIdx.x; b < bt.n; b += blockDim.x)
-      if (bt.cu[b] <= t && t < bt.cu[b + 1]) atomicMax(slot, b);
-  } else if (threadIdx.x == 0 && t < bt.n) {
-    *slot = t;
-  }
-  __syncthreads();
-  const int b = *slot;
-  if (b < 0) return r;
-  const KvSeq s = kv_seq(c, bt, b);
-  int twice = 0;
-  if (bt.seqs)
-    for (int i = threadIdx.x; i < b; i += blockDim.x) twice |= bt.seqs[i] == s.s;
-  twice = __syncthreads_or(twice);
-  if (s.s < 0 || twice) {
-    if (threadIdx.x == 0) atomicOr(c.status, kKvBadSeq);
-    return r;
-  }
-  r.seq = s.s;
-  r.pos = s.len - s.nq + (t - s.q0);
-  r.ok = true;
-  return r;
+// The sum of squares of a head, from its lanes' eight features each.
+template <int LPR>
+__device__ __forceinline__ float group_sum(const float (&f)[8]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  return ss;
 }
+
+// Where the token of a CTA belongs.
+struct KvToken {
+  int entry;      // of the batch, -1: behind the last sequence
+  int seq, pos;   // row of the page table (-1: no such), position (negative: fewer tokens held than new)
+  int64_t place;  // row of its kv head 0 in a layer's pool, -1: none
+};
 
 // cos and sin of pos * inv_freq[j].
 __device__ __forceinline__ float2 kv_angle(int pos, float inv_freq) {
@@ -129,91 +120,201 @@ __device__ __forceinline__ float2 kv_angle(int pos, float inv_freq) {
   return r;
 }
 
-// Place of kv head 0 of the token in a layer's pool, or -1 without one.
-__device__ __forceinline__ int64_t kv_place(const KvView& c, const KvToken& tk) {
-  if (tk.pos < 0) {
-    if (threadIdx.x == 0) atomicOr(c.status, kKvBadPage);
-    return -1;
+// All threads: finds token t, and in the same two block barriers fills cs with
+// the cosines and sines of its rot / 2 angles.  An entry whose sequence stands
+// earlier in the list as well is refused (two entries would write the same
+// places).  False: nothing to do.
+__device__ __forceinline__ bool kv_find_token(const KvAppend& a, int t, KvToken* sh, float2* cs) {
+  const KvView& c = a.c;
+  const KvBatch& bt = a.bt;
+  // every thread looks at its entries at once; the one that has the token
+  // goes on to its length (the entries are apart, so no two match unless cu
+  // is not increasing: then any of them)
+  if (threadIdx.x == 0) sh->entry = -1;
+  __syncthreads();
+  int my_seq = -1;  // of the last entry that this thread looked at
+  for (int b = threadIdx.x; b < bt.n; b += blockDim.x) {
+    const int q0 = bt.cu ? bt.cu[b] : b, q1 = bt.cu ? bt.cu[b + 1] : b + 1;
+    my_seq = bt.seqs ? bt.seqs[b] : b;
+    if (q0 <= t && t < q1) {
+      const KvSeq s = kv_seq(c, bt, b);
+      sh->seq = s.s;
+      sh->pos = s.len - s.nq + (t - s.q0);
+      sh->entry = b;
+    }
   }
-  const int page = c.table[(size_t)tk.seq * c.max_pages + (tk.pos >> c.ps_shift)];
-  if (page < 0 || page >= c.pages) {
-    if (threadIdx.x == 0) atomicOr(c.status, kKvBadPage);
-    return -1;
+  __syncthreads();
+  const int entry = sh->entry, seq = sh->seq, pos = sh->pos;
+  if (entry < 0) return false;
+  int twice = 0;
+  if (bt.seqs) {
+    if (bt.n <= (int)blockDim.x) {
+      twice = (int)threadIdx.x < entry && my_seq == seq;
+    } else {
+      for (int b = threadIdx.x; b < entry; b += blockDim.x) twice |= bt.seqs[b] == seq;
+    }
   }
-  return ((int64_t)page * c.hk << c.ps_shift) + (tk.pos & ((1 << c.ps_shift) - 1));  // in rows of head_dim
+  if (threadIdx.x < a.rot / 2) cs[threadIdx.x] = kv_angle(pos, a.inv_freq[threadIdx.x]);
+  if (threadIdx.x == blockDim.x - 1) {
+    int page = -1;
+    if (seq >= 0 && pos >= 0) page = c.table[(size_t)seq * c.max_pages + (pos >> c.ps_shift)];
+    const bool there = page >= 0 && page < c.pages;
+    sh->place = there ? ((int64_t)page * c.hk << c.ps_shift) + (pos & ((1 << c.ps_shift) - 1)) : -1;
+    if (seq >= 0 && !there) atomicOr(c.status, kKvBadPage);
+  }
+  twice = __syncthreads_or(twice);
+  if (seq < 0 || twice) {
+    if (threadIdx.x == 0) atomicOr(c.status, kKvBadSeq);
+    return false;
+  }
+  return true;
 }
 
 // blockIdx.x = token, blockIdx.y = share of its rows (heads of q, k and v).
 // LPR lanes per row, head_dim and rot_dim multiples of 8, rows of the inputs
-// and pools aligned to 4 elements.
+// and pools aligned to 4 elements.  For few tokens: each thread has one octet,
+// requested first, so that it is on its way while the token's place is looked up.
 template <typename T, int LPR, bool SPLIT>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppend a) {
-  __shared__ int slot;
+  __shared__ KvToken token;
   __shared__ float2 cs[128];
+  using Oct = Octet<T, SPLIT>;
   pdl_wait();
   const KvView& c = a.c;
-  const int t = blockIdx.x, d = c.d;
-  const KvToken tk = kv_find_token(c, a.bt, t, &slot);
-  if (!tk.ok) return;
-  if (threadIdx.x < a.rot / 2) cs[threadIdx.x] = kv_angle(tk.pos, a.inv_freq[threadIdx.x]);
-  const int64_t place = kv_place(c, tk);
-  __syncthreads();
-  const int rows = a.hq + 2 * c.hk, u = threadIdx.x % LPR;
+  const int t = blockIdx.x, d = c.d, rows = a.hq + 2 * c.hk, u = threadIdx.x % LPR;
   const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(rows, row0 + a.rows_per_cta);
+  const int r = row0 + threadIdx.x / LPR;  // rows_per_cta: one row a group of lanes
+  const bool live = 8 * u < d && r < row1;
+  const bool is_q = r < a.hq, is_k = !is_q && r < a.hq + c.hk;
+  const int h = is_q ? r : is_k ? r - a.hq : r - a.hq - c.hk;
+  const int rot = is_q || is_k ? a.rot : 0;
+  const T* w = static_cast<const T*>(is_q ? a.qw : is_k ? a.kw : nullptr);
+  typename Oct::Raw raw, rw;
+  if (live) {
+    const T* x = is_q   ? static_cast<const T*>(a.q) + (int64_t)t * a.qs
+                 : is_k ? static_cast<const T*>(a.k) + (int64_t)t * a.ks
+                        : static_cast<const T*>(a.v) + (int64_t)t * a.vs;
+    Oct::load(x + (int64_t)h * d, u, rot, raw);
+    if (w) Oct::load(w, u, rot, rw);
+  }
+  if (!kv_find_token(a, t, &token, cs)) return;
+  const int64_t place = token.place;
+  float f[8] = {};
+  if (live) Oct::values(raw, f);
+  const float ss = group_sum<LPR>(f);
+  if (!live || (!is_q && place < 0)) return;
+  if (w) Oct::norm(f, rsqrtf(ss / (float)d + a.eps), rw);
+  if (8 * u < rot) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) Oct::turn(f, e, cs[4 * u + e]);
+  }
+  T* y = is_q ? static_cast<T*>(a.qo) + (int64_t)t * a.os + (int64_t)h * d
+              : static_cast<T*>(is_k ? c.k : c.v) + a.layer_off + (size_t)(place + ((int64_t)h << c.ps_shift)) * d;
+  Oct::store(y, u, rot, f);
+}
+
+// The same for many tokens: a warp a token, nothing shared, no barrier.  A
+// lane's place within a head is the same for all heads, so it keeps the norms'
+// weights and the cosines and sines of its four pairs in registers, and the
+// rows of a token are one stream of loads with the lookup behind the first.
+template <typename T, int LPR, bool SPLIT>
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_warp_kernel(KvAppend a) {
+  using Oct = Octet<T, SPLIT>;
+  pdl_wait();
+  const KvView& c = a.c;
+  const int lane = threadIdx.x & 31, u = lane % LPR, d = c.d;
+  const int t = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  if (t >= a.bt.total) return;
+  constexpr int RPS = 32 / LPR, AT_ONCE = sizeof(T) == 4 ? 3 : 4;  // rows a step, steps a request
+  typename Oct::Raw raw[AT_ONCE];
   const bool mine = 8 * u < d;
-  constexpr int STEP = kAppendThreads / LPR;
-  // whole warps iterate, so that the shuffles below have all their lanes
-  for (int r0 = row0; r0 < row1; r0 += STEP) {
-    const int r = r0 + threadIdx.x / LPR;
-    const bool live = mine && r < row1;
-    const bool is_q = r < a.hq, is_k = !is_q && r < a.hq + c.hk;
-    const int h = is_q ? r : is_k ? r - a.hq : r - a.hq - c.hk;
-    const T* x = is_q ? static_cast<const T*>(a.q) + (int64_t)t * a.qs
-                      : is_k ? static_cast<const T*>(a.k) + (int64_t)t * a.ks : static_cast<const T*>(a.v) + (int64_t)t * a.vs;
-    const int rot = is_q || is_k ? a.rot : 0;
-    float f[8] = {};
-    if (live) Octet<T, SPLIT>::load(x + (int64_t)h * d, u, rot, f);
-    const T* w = static_cast<const T*>(is_q ? a.qw : is_k ? a.kw : nullptr);
-    float ss = 0.0f;
+  const int first = lane / LPR;
+  auto request = [&](const T* x, int r0, int n, int rot) {  // of n heads at x
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) continue;
-    if (w) {
-      const float inv = rsqrtf(ss / (float)d + a.eps);
-      float wf[8];
-      Octet<T, SPLIT>::load(w, u, rot, wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * wf[i];
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int r = r0 + i * RPS + first;
+      if (mine && r < n) Oct::load(x + r * d, u, rot, raw[i]);
     }
-    if (8 * u < rot) {
-      if constexpr (SPLIT) {
+  };
+  const T* xq = static_cast<const T*>(a.q) + (int64_t)t * a.qs;
+  request(xq, 0, a.hq, a.rot);
+  // the last entry that begins at or before the token: 32 candidates a round
+  const KvBatch& bt = a.bt;
+  int entry = t;
+  if (bt.cu) {
+    entry = 0;
+    for (int size = bt.n; size > 1;) {
+      const int stride = (size + 31) / 32, b = entry + lane * stride;
+      const uint32_t before = __ballot_sync(0xffffffffu, lane * stride < size && bt.cu[b] <= t);
+      const int k = before ? 31 - __clz(before) : 0;
+      size = min(stride, size - k * stride);
+      entry += k * stride;
+    }
+    if (!(bt.cu[entry] <= t && t < bt.cu[entry + 1])) return;  // behind the last sequence
+  } else if (t >= bt.n) {
+    return;
+  }
+  const KvSeq s = kv_seq(c, bt, entry);
+  const int pos = s.len - s.nq + (t - s.q0);
+  bool twice = false;
+  if (bt.seqs)
+    for (int b = lane; b < entry; b += 32) twice |= bt.seqs[b] == s.s;
+  int page = -1;
+  if (s.s >= 0 && pos >= 0) page = c.table[(size_t)s.s * c.max_pages + (pos >> c.ps_shift)];
+  if (__any_sync(0xffffffffu, twice) || s.s < 0) {
+    if (lane == 0) atomicOr(c.status, kKvBadSeq);
+    return;
+  }
+  const bool there = page >= 0 && page < c.pages;
+  if (!there && lane == 0) atomicOr(c.status, kKvBadPage);
+  const int64_t place = ((int64_t)page * c.hk << c.ps_shift) + (pos & ((1 << c.ps_shift) - 1));
+  float2 cs[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 e = cs[4 * u + i];
-          const float p = f[i], q = f[i + 4];
-          f[i] = p * e.x - q * e.y;
-          f[i + 4] = q * e.x + p * e.y;
-        }
-      } else {
+  for (int e = 0; e < 4; ++e)
+    if (8 * u < a.rot) cs[e] = kv_angle(pos, a.inv_freq[4 * u + e]);
+  const float per_d = 1.0f / (float)d;
+  // n heads at x, norm and rotation, to y, `step` apart
+  auto turn = [&](const T* x, T* y, int n, int64_t step, const T* weight, bool asked) {
+    float w[8];
+    if (weight && mine) {
+      typename Oct::Raw rw;
+      Oct::load(weight, u, a.rot, rw);
+      Oct::values(rw, w);
+    }
+    for (int r0 = 0; r0 < n; r0 += AT_ONCE * RPS) {
+      if (!asked || r0 > 0) request(x, r0, n, a.rot);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 e = cs[4 * u + i];
-          const float p = f[2 * i], q = f[2 * i + 1];
-          f[2 * i] = p * e.x - q * e.y;
-          f[2 * i + 1] = q * e.x + p * e.y;
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (r0 + i * RPS >= n) break;
+        const int r = r0 + i * RPS + first;
+        const bool live = mine && r < n;
+        float f[8] = {};
+        if (live) Oct::values(raw[i], f);
+        if (weight) {
+          const float inv = rsqrtf(fmaf(group_sum<LPR>(f), per_d, a.eps));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = f[e] * inv * w[e];
         }
+        if (8 * u < a.rot)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) Oct::turn(f, e, cs[e]);
+        if (live) Oct::store(y + r * step, u, a.rot, f);
       }
     }
-    T* y;
-    if (is_q) {
-      y = static_cast<T*>(a.qo) + (int64_t)t * a.os + (int64_t)h * d;
-    } else {
-      if (place < 0) continue;
-      y = static_cast<T*>(is_k ? c.k : c.v) + a.layer_off + (size_t)(place + ((int64_t)h << c.ps_shift)) * d;
+  };
+  turn(xq, static_cast<T*>(a.qo) + (int64_t)t * a.os, a.hq, d, static_cast<const T*>(a.qw), true);
+  if (!there) return;
+  const int64_t head = (int64_t)d << c.ps_shift;
+  turn(static_cast<const T*>(a.k) + (int64_t)t * a.ks, static_cast<T*>(c.k) + a.layer_off + place * d, c.hk, head, static_cast<const T*>(a.kw), false);
+  const T* xv = static_cast<const T*>(a.v) + (int64_t)t * a.vs;
+  T* yv = static_cast<T*>(c.v) + a.layer_off + place * d;
+  for (int r0 = 0; r0 < c.hk; r0 += AT_ONCE * RPS) {
+    request(xv, r0, c.hk, 0);
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int r = r0 + i * RPS + first;
+      if (mine && r < c.hk) Oct::store(yv + r * head, u, 0, raw[i]);
     }
-    Octet<T, SPLIT>::store(y, u, rot, f);
   }
 }
 
@@ -222,16 +323,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppend a) {
 // the remaining features two by two.
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_any_kernel(KvAppend a, int interleaved) {
-  __shared__ int slot;
+  __shared__ KvToken token;
   __shared__ float2 cs[128];
   pdl_wait();
   const KvView& c = a.c;
   const int t = blockIdx.x, d = c.d;
-  const KvToken tk = kv_find_token(c, a.bt, t, &slot);
-  if (!tk.ok) return;
-  if (threadIdx.x < a.rot / 2) cs[threadIdx.x] = kv_angle(tk.pos, a.inv_freq[threadIdx.x]);
-  const int64_t place = kv_place(c, tk);
-  __syncthreads();
+  if (!kv_find_token(a, t, &token, cs)) return;
+  const int64_t place = token.place;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row0 = blockIdx.y * a.rows_per_cta, row1 = min(a.hq + 2 * c.hk, row0 + a.rows_per_cta);
   for (int r = row0 + warp; r < row1; r += kAppendThreads / 32) {
@@ -297,28 +395,31 @@ static int launch_append(KvAppend a, int interleaved, cudaStream_t s) {
                    quad(a.c.v) && quad(a.qw) && quad(a.kw) && a.qs % 4 == 0 && a.ks % 4 == 0 && a.vs % 4 == 0 && a.os % 4 == 0;
   const int lpr = !vec ? 32 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
   const int step = kAppendThreads / lpr, steps = (rows + step - 1) / step;
-  // few tokens: a token's rows over several CTAs, each with one step of them
-  // (one token of 36 heads: 3 CTAs); many: one CTA, its angles computed once
+  // few tokens: a token's rows over several CTAs, a step of them each (one
+  // token of 36 heads: 3 CTAs, 3.1 us; a warp for it: 6); many: a warp a token
   const bool spread = (int64_t)a.bt.total * steps <= 4 * (int64_t)std::max(1, sm_count());
-  const int shares = spread ? steps : 1;
   a.rows_per_cta = spread ? step : rows;
-  const dim3 grid(a.bt.total, shares), block(kAppendThreads);
-  auto go = [&](auto kern) {
+  const dim3 block(kAppendThreads);
+  auto go = [&](auto kern, dim3 grid) {
     OC_CHECK_CUDA(launch_pdl_ex(kern, grid, block, 0, s, a));
     return OC_OK;
   };
   if (!vec) {
-    OC_CHECK_CUDA(launch_pdl_ex(kv_append_any_kernel<T>, grid, block, 0, s, a, interleaved));
+    OC_CHECK_CUDA(launch_pdl_ex(kv_append_any_kernel<T>, dim3(a.bt.total, spread ? steps : 1), block, 0, s, a, interleaved));
     return OC_OK;
   }
-  if (interleaved) {
-    if (lpr == 8) return go(kv_append_kernel<T, 8, false>);
-    if (lpr == 16) return go(kv_append_kernel<T, 16, false>);
-    return go(kv_append_kernel<T, 32, false>);
-  }
-  if (lpr == 8) return go(kv_append_kernel<T, 8, true>);
-  if (lpr == 16) return go(kv_append_kernel<T, 16, true>);
-  return go(kv_append_kernel<T, 32, true>);
+  auto pick = [&](auto lanes, auto split) {
+    constexpr int LPR = decltype(lanes)::value;
+    constexpr bool SPLIT = decltype(split)::value;
+    if (spread) return go(kv_append_kernel<T, LPR, SPLIT>, dim3(a.bt.total, steps));
+    return go(kv_append_warp_kernel<T, LPR, SPLIT>, dim3((a.bt.total + kAppendThreads / 32 - 1) / (kAppendThreads / 32)));
+  };
+  auto by_style = [&](auto lanes) {
+    return interleaved ? pick(lanes, std::false_type()) : pick(lanes, std::true_type());
+  };
+  if (lpr == 8) return by_style(std::integral_constant<int, 8>());
+  if (lpr == 16) return by_style(std::integral_constant<int, 16>());
+  return by_style(std::integral_constant<int, 32>());
 }
 
 }  // namespace oc

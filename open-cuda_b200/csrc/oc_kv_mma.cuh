@@ -58,24 +58,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// {a, b} rounded to T and packed (a in the low half).
-template <typename T>
-__device__ __forceinline__ uint32_t kv_pack2(float a, float b) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ float2 kv_unpack2(uint32_t x) {
-  if constexpr (std::is_same<T, __half>::value)
-    return __half22float2(*reinterpret_cast<__half2*>(&x));
-  else
-    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-}
-
 // One row of one query head from the definition, by one warp: for rows whose
 // result is not finite.  Reads only keys that the row sees.
 template <typename T>
