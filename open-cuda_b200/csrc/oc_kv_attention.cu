@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, KvParts parts, 
     // piece 0 is in slot 1 of that CTA, piece i in slot 0 of the i-th behind it
     const float* first = pt.ws + plan_cut_floats(pt.ctas) + (size_t)cta * step + slot;
     const float* rest = first + slot;
-    constexpr int U = R == 1 ? 4 : 2;
+    constexpr int U = R == 1 ? 8 : 2;
     float m = -INFINITY, l = 0.0f;
     float4 acc[NV] = {};  // features 4 lane .. (and 128 + 4 lane ..)
     for (int i0 = warp % SPLIT; i0 < pieces; i0 += SPLIT * U) {
@@ -219,7 +219,7 @@ static KvLaunch scalar_launch(int d, int rows) {
 // On warp-level matrix instructions.
 template <typename T>
 static KvLaunch mma_launch(int d, int rows) {
-  auto go = [](auto k) { return shape_of<decltype(k)>(kv_mma_kernel<decltype(k)>, 2); };
+  auto go = [](auto k) { return shape_of<decltype(k)>(kv_mma_kernel<decltype(k)>, 1); };
   if (d <= 64) return rows <= 16 ? go(KvMma<T, 64, 1>()) : go(KvMma<T, 64, 2>());
   if (d <= 96) return rows <= 16 ? go(KvMma<T, 96, 1>()) : go(KvMma<T, 96, 2>());
   if (d <= 128) return rows <= 16 ? go(KvMma<T, 128, 1>()) : go(KvMma<T, 128, 2>());
@@ -250,7 +250,11 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
       out[1] = c.d == 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
     }
   } else {
-    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, tile ? kFewRows : likely) : scalar_launch<T>(c.d, likely);
+    // beside chunks that go to the tiles the few rows are mostly single tokens'
+    // (16 rows an item), unless the whole batch is of a few tokens each
+    const int64_t mean = (int64_t)tokens * group / std::max(1, n);
+    const int few = mean <= 2 * kFewRows ? kFewRows : std::min(kFewRows, group);
+    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, tile ? few : likely) : scalar_launch<T>(c.d, likely);
     if (tile) {
       auto go = [](auto k) {
         KvLaunch l = shape_of<decltype(k)>(nullptr, 2);

@@ -101,6 +101,31 @@ __device__ __forceinline__ int64_t plan_head_block(const KvPlan& p, const KvSeq&
 // many row blocks (a chunk of 2048 tokens has hundreds) are summed by all.
 __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c, const KvBatch& bt, int index,
                                                KvPlanShared* sh, int64_t* chunk, KvCursor& cur) {
+  if (bt.n == 1) {  // one sequence of few row blocks: every thread sees all there is
+    const KvSeq s = kv_seq(c, bt, 0);
+    const int blocks = plan_blocks(p, s);
+    if (blocks == 0) return 0;
+    if (blocks <= kPlanSmall) {
+      int64_t head = 0;
+      for (int j = 0; j < blocks; ++j) head += plan_item(p, s, j).units;
+      const int64_t all = head * c.hk;
+      *chunk = max((int64_t)p.min_units, (all + p.ctas - 1) / p.ctas);
+      int64_t off = *chunk * index;
+      if (off >= all) return 0;
+      cur.b = 0;
+      cur.s = s;
+      cur.blocks = blocks;
+      cur.h = (int)(off / head);
+      off -= cur.h * head;
+      for (cur.j = 0;; ++cur.j) {
+        cur.it = plan_item(p, s, cur.j);
+        if (off < cur.it.units) break;
+        off -= cur.it.units;
+      }
+      cur.at = (int)off;
+      return all;
+    }
+  }
   int64_t total = 0, u;
   bool have = false;
   if (threadIdx.x == 0) sh->b = -1;

@@ -128,31 +128,11 @@ __device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, 
   return true;
 }
 
-// fa_max_chunk and fa_p_chunk for a row that sees keys [from, to) of the chunk.
-__device__ __forceinline__ float kv_max_chunk(const uint32_t (&r)[32], const float* ik, int from, int to, float tmax) {
+// Scores outside [from, to) of a 32-key chunk become `out`.
+__device__ __forceinline__ void kv_mask_chunk(uint32_t (&r)[32], int from, int to, uint32_t out) {
 #pragma unroll
   for (int j = 0; j < 32; ++j)
-    if (j >= from && j < to) tmax = fmaxf(tmax, __fmul_rn(__uint_as_float(r[j]), ik[j]));
-  return tmax;
-}
-__device__ __forceinline__ float kv_p_chunk(const uint32_t (&r)[32], const float* ik, float rq2, float nb, int from, int to,
-                                            uint32_t (&ph16)[16], uint32_t (&pl16)[16]) {
-  float psum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    float p[2], h[2], l[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float x = __fmaf_rn(__fmul_rn(__uint_as_float(r[j + u]), ik[j + u]), rq2, nb);
-      // (a NaN goes through: fminf would drop it)
-      p[u] = j + u >= from && j + u < to ? fa_ex2(x > 15.0f ? 15.0f : x) : 0.0f;
-      psum = __fadd_rn(psum, p[u]);
-      fa_split(p[u], h[u], l[u]);
-    }
-    ph16[j >> 1] = fa_pack_f16x2(h[0], h[1]);
-    pl16[j >> 1] = fa_pack_f16x2(l[0], l[1]);
-  }
-  return psum;
+    if (j < from || j >= to) r[j] = out;
 }
 
 template <typename K>
@@ -320,6 +300,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
   } else if (warp <= kFaConv + 4) {
     const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t unseen = a.scale2 < 0.0f ? 0x7f800000u : 0xff800000u;  // minus infinity once it has the key factors' sign
     bool ok = true;
     uint32_t n = 0, items = 0;
     for (;;) {
@@ -327,14 +308,14 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
       ok = jobs.template take<true>(it, abort_flag);
       const int t0 = it.t0, t1 = it.t1;
       if (!ok || t0 == t1) break;
-      int lo = 0, hi = 0;
-      if (row < it.rows) plan_row_range(a.p, it.s, it.r0 + row, lo, hi);
+      int lo, hi;  // (rows behind the last see what it sees: masks are a whole warp's affair)
+      plan_row_range(a.p, it.s, it.r0 + min(row, it.rows - 1), lo, hi);
       float rq2 = 0.0f;
       float m_i = -INFINITY, l_i = 0.0f;  // running max (log2 units) and 2^15-scaled sum
       for (int t = t0; t < t1; ++t, ++n) {
         const uint32_t ph = n & 1u;
         const int key0 = (it.tile0 + t) * K::BK, from = lo - key0, to = hi - key0;  // keys of this tile that are seen
-        const bool all = from <= 0 && to >= K::BK;
+        const bool all = __all_sync(0xffffffffu, from <= 0 && to >= K::BK);
         const float* ik = sh.ick[ph];
         ok = warp_wait(&sh.s_full, ph, abort_flag);
         if (!ok) break;
@@ -342,26 +323,25 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
         // |scale| * log2(e) / c_q; the sign of scale rides on the key factors.
         // (S was computed from the queries, so their factors are there too; the
         // barrier of the queries may be phases ahead of this warp by now.)
-        if (t == t0) rq2 = __fmul_rn(fabsf(a.scale2), sh.icq[items & 1][row]);
-        // pass 1: the tile's max of S' * sign / c_k (rq2 >= 0 keeps the order)
+        // (A scale of zero as the least that keeps minus infinity what it is.)
+        if (t == t0) rq2 = fmaxf(__fmul_rn(fabsf(a.scale2), sh.icq[items & 1][row]), 1.2e-38f);
+        // pass 1: the tile's max of S' * sign / c_k (rq2 > 0 keeps the order)
         float tmax = -INFINITY;
 #pragma unroll 1
         for (int cb = 0; cb < 4; ++cb) {
           uint32_t r[32];
           tmem_ld32(lanes + K::S_COL + cb * 32, r);
           tmem_ld_wait();
-          tmax = all ? fa_max_chunk<false>(r, ik + cb * 32, 32, tmax) : kv_max_chunk(r, ik + cb * 32, from - cb * 32, to - cb * 32, tmax);
+          if (!all) kv_mask_chunk(r, from - cb * 32, to - cb * 32, unseen);
+          tmax = fa_max_chunk<false>(r, ik + cb * 32, 32, tmax);
         }
         const float tm = tmax == -INFINITY ? -INFINITY : __fmul_rn(tmax, rq2);
         const float new_m = fmaxf(m_i, tm);
         const float corr = (m_i == -INFINITY) ? 0.0f : fa_ex2(__fsub_rn(m_i, new_m));
-        // pass 2: p, the tile's sum, P terms into tensor memory.  Past |m'| =
-        // 2^20 the rounding of 15 - m' can reach an exponent above 15, so that
-        // range (and partly visible tiles) takes the guarded path.
-        const bool dead = new_m == -INFINITY;
-        const bool guard = dead || !all || fabsf(new_m) > 1048576.0f;
-        const float nb = dead ? 0.0f : __fsub_rn(15.0f, new_m);
-        const int f2 = dead ? 0 : from, e2 = dead ? 0 : to;
+        // pass 2: p, the tile's sum, P terms into tensor memory.  (Past |m'| =
+        // 2^20 the rounding of 15 - m' can reach an exponent of 16, which no
+        // f16 holds: such a row is not finite and computed again.)
+        const float nb = new_m == -INFINITY ? 0.0f : __fsub_rn(15.0f, new_m);
         float psum = 0.0f;
 #pragma unroll 1
         for (int cb = 0; cb < 4; ++cb) {
@@ -369,8 +349,8 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
           tmem_ld32(lanes + K::S_COL + cb * 32, r);
           tmem_ld_wait();
           uint32_t ph16[16], pl16[16];
-          psum = __fadd_rn(psum, guard ? kv_p_chunk(r, ik + cb * 32, rq2, nb, f2 - cb * 32, e2 - cb * 32, ph16, pl16)
-                                       : fa_p_chunk<false>(r, ik + cb * 32, rq2, nb, 32, ph16, pl16));
+          if (!all) kv_mask_chunk(r, from - cb * 32, to - cb * 32, unseen);
+          psum = __fadd_rn(psum, fa_p_chunk<false>(r, ik + cb * 32, rq2, nb, 32, ph16, pl16));
           // over S' chunk cb, which this thread has read
           tmem_st16(lanes + K::S_COL + cb * 32, ph16);
           tmem_st16(lanes + K::S_COL + cb * 32 + 16, pl16);
