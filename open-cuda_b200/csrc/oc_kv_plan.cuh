@@ -78,7 +78,7 @@ struct KvCursor {
   int at;           // unit within the item
 };
 
-constexpr int kPlanSmall = 8;  // row blocks that one thread sums by itself
+constexpr int kPlanSmall = 32;  // row blocks that one thread sums by itself (the threads do it side by side)
 
 struct KvPlanShared {
   int64_t sums[33];
@@ -105,7 +105,7 @@ __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c,
     const KvSeq s = kv_seq(c, bt, 0);
     const int blocks = plan_blocks(p, s);
     if (blocks == 0) return 0;
-    if (blocks <= kPlanSmall) {
+    if (blocks <= 8) {
       int64_t head = 0;
       for (int j = 0; j < blocks; ++j) head += plan_item(p, s, j).units;
       const int64_t all = head * c.hk;

@@ -7,14 +7,22 @@
 //   P = 2^(scale2 * S - m)               (softmax warps, TMEM -> TMEM)
 //   O += P V       128 x d, K = 128 keys (P in tensor memory over S's
 //                  columns, V in shared memory, read as rows of keys)
-// Bound: a tile is 2 * 2 * 128 * 128 * d multiply-adds per sub-tile (2048
-// cycles of the tensor pipe for both at d = 128) and 2 * 16384 exponentials
-// (2048 cycles at 16 a clock), so neither may wait for the other: while one
-// sub-tile's softmax runs, the tensor cores do the other's products.  O stays
-// in tensor memory and is rescaled only when a row's maximum grows by more
-// than 2^8 since the last time (weights up to 2^8 are exact powers away from
-// the usual ones, and both types hold them): after the first tiles that is
-// rare, so the softmax almost never waits for the accumulator.
+// Bound: a tile's products take 2200 cycles of the tensor pipe at d = 128 (69
+// an instruction measured, 32 of them) and its 2 * 16384 exponentials 2048 of
+// the transcendental units, so neither may wait for the other: while one
+// sub-tile's softmax runs, the tensor cores do the other's products, and the
+// product with V begins on three quarters of the weights.  What is left is
+// the chain of a sub-tile (scores out of tensor memory 420 cycles, maximum
+// 370, exponentials 1500, then its two products): 3900 cycles a tile by a
+// clock record.  Measured: chunks of 1.9 to 2 k tokens over 14 to 16 k keys,
+// 32 heads of 128 over 8, 930 to 1010 us = 0.9 to 0.98 PFLOP/s.  Not kept, all slower there:
+// two threads a row (16 softmax warps, 96 registers: 1120 us), exponentials
+// in part as polynomials on the multiply-add pipe (1060 to 1200), items of 128
+// rows whose tiles two softmax groups take in turn (1215: twice the keys'
+// traffic).  O stays in tensor memory and is rescaled only when a row's
+// maximum grows by more than 2^8 since the last time (weights up to 2^8 lose
+// nothing in either type): after the first tiles that is rare, so the softmax
+// almost never waits for the accumulator.
 //
 // 384 threads, one CTA an SM:
 //   warp 0       TMEM allocator, MMA issuer (lane 0)

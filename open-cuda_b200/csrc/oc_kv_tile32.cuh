@@ -3,17 +3,20 @@
 //
 // The arithmetic is flash_tc_kernel's (oc_flash_tc.cuh): every operand as two
 // f16 terms of a power-of-two scaling (Q and K per row, V per tile, P by
-// 2^15), three MMAs per product step (the small terms first), scores in log2 units, the running output
-// rescaled with every tile.  What differs is where rows come from and how the
+// 2^15), three MMAs per product step (the small terms first), scores in log2
+// units, the running output rescaled with every tile.  What differs is where rows come from and how the
 // work is shared out: query rows are the heads of a kv head of consecutive
 // tokens, key rows are looked up page by page (zeros where no row of the item
 // sees a key), a CTA works through a run of pieces (oc_kv_plan.cuh), and what
 // a cut leaves goes to the workspace.
 //
-// Bound: the conversion of K and V (each element once per item: two f16 terms
-// take about ten instructions a pair) and the chain S -> softmax -> P V of a
-// tile, not the tensor pipe; 8 prompts of 300 to 777 tokens over 12 heads of
-// 64 measured: see the table of the operators.
+// Bound: not the tensor pipe but the chain of a tile, S -> softmax (two passes
+// over tensor memory) -> P V -> next S, about 8000 cycles at d = 64, and the
+// conversion of K and V beside it.  Measured: 8 prompts of 300 to 777 tokens
+// over contexts of 800 to 1000, 12 heads of 64: 143 us a call (55 TFLOP/s of
+// visible products; the CUDA cores took 1220).  S in two buffers with K
+// converted a tile ahead measured slower (167 us: the softmax warps, which
+// share their schedulers with the converters, spill).
 //
 // One CTA an SM, 448 threads:
 //   warp 0       TMEM allocator + MMA issuer (lane 0)

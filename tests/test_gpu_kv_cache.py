@@ -225,6 +225,23 @@ def test_unaligned_queries_and_pools(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("new", [[1, 1], [1, 90], [90, 200]])
+def test_unaligned_outputs(dtype, d, new):
+    """Results to rows that no vector store can take, and to odd pairs."""
+    c, ks, vs = filled(dtype, 2, d, 16, [400, 999])
+    m = sum(new)
+    q = torch.randn(m, 4, d, device="cuda").to(dtype)
+    want, tol = expected(q, ks, vs, [0, 1], new, 1 / math.sqrt(d), True, 0)
+    for gap in (1, 2):
+        raw = torch.full((m * (4 * d + gap) + gap,), 7.0, dtype=dtype, device="cuda")
+        out = raw.as_strided((m, 4, d), (4 * d + gap, d, 1), gap)
+        attend(c, q, [0, 1], new, out=out)
+        close(out, want, tol)
+        assert (raw[:gap] == 7).all() and (raw[gap:].view(m, 4 * d + gap)[:, 4 * d:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 96, 128])
 def test_rows_without_keys_are_zero(dtype, d):
     """No keys at all, and more new tokens than the sequence holds: the first
@@ -406,17 +423,21 @@ def rotated(x, pos, inv, interleaved):
     return y, size
 
 
+LENS, NEW = [1, 33, 100, 20000], [1, 20, 0, 7]
+MANY = [1, 900, 100, 20000], [1, 700, 0, 60]  # enough tokens for a warp each
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens, new", [(LENS, NEW), MANY])
 @pytest.mark.parametrize("hq, hk, d, rot", [(28, 4, 128, 128), (12, 12, 64, 64), (8, 2, 80, 80), (6, 2, 96, 32), (4, 4, 256, 256), (3, 3, 17, 10),
                                             (2, 1, 250, 250), (5, 5, 40, 12), (8, 8, 64, 0), (0, 2, 128, 64), (4, 2, 8, 8), (70, 10, 128, 128)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("norm", [False, True])
-def test_append(dtype, hq, hk, d, rot, interleaved, norm):
+def test_append(dtype, lens, new, hq, hk, d, rot, interleaved, norm):
     """Error: one rounding, and in f32 before it d + 10 units of the norm's
     sum and factors, 4 for the rotation and 2^-22 for its cosines (a turn is
     reduced in f64 and given to f32 within 2^-25, times 2 pi): of the sizes
     that are summed."""
-    lens, new = [1, 33, 100, 20000], [1, 20, 0, 7]
     c, _, _ = filled(dtype, hk, d, 16, lens, layers=2, layer=1, seed=d)
     m = sum(new)
     buf = torch.randn(m + 2, hq + 2 * hk + 1, d, device="cuda").to(dtype)[:m]
@@ -455,6 +476,31 @@ def test_append(dtype, hq, hk, d, rot, interleaved, norm):
         assert torch.equal(torch.nan_to_num(x, 9.0), torch.nan_to_num(y, 9.0))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens", [40, 900])
+def test_append_of_many_sequences(dtype, tokens):
+    """More sequences than a warp has lanes, with and without cu, in place."""
+    hq, hk, d = 6, 2, 64
+    lens = [1 + (5 * i) % 37 for i in range(tokens)]
+    c, _, _ = filled(dtype, hk, d, 8, lens, seed=tokens)
+    x = torch.randn(tokens, hq + 2 * hk, d, device="cuda").to(dtype)
+    ids = list(np.random.default_rng(0).permutation(tokens))
+    inv = (10000.0 ** (-torch.arange(0, d, 2, device="cuda").double() / d)).float()
+    pos = torch.tensor([lens[s] - 1 for s in ids], device="cuda")
+    y, size = rotated(x[:, :hq].double(), pos, inv, False)
+    tol = HALF_STEP[dtype] * y.abs() + size * 8.1 * 2.0 ** -24 + SMALLEST[dtype]
+    outs = []
+    for cu in (None, ints(range(tokens + 1))):
+        outs.append(c.append(0, x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:], cu, ints(ids), inv_freq=inv))
+        close(outs[-1], y, tol)
+    assert torch.equal(outs[0], outs[1])
+    page = c.page_table[torch.tensor(ids, device="cuda"), pos // 8].long()
+    assert torch.equal(c.v[0][page, :, pos % 8], x[:, hq + hk:])
+    c.append(0, x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:], None, ints(ids), inv_freq=inv, q_out=x[:, :hq])
+    assert torch.equal(x[:, :hq], outs[0])
+    c.check()
+
+
 def test_append_in_place_unaligned_and_far():
     for dtype in (F32, F16, BF16):
         c, _, _ = filled(dtype, 2, 64, 1024, [1], spare=0)
@@ -471,13 +517,15 @@ def test_append_in_place_unaligned_and_far():
         c.check()
 
 
-def test_append_refusals_on_the_device():
+@pytest.mark.parametrize("behind", [0, 1000])
+def test_append_refusals_on_the_device(behind):
+    """Few tokens, and the same six in front of a thousand that no sequence has."""
     for dtype, d in ((F16, 64), (F32, 17)):
         c, _, _ = filled(dtype, 2, d, 16, [40, 50])
-        x = torch.randn(6, 6, d, device="cuda").to(dtype)
+        x = torch.randn(6 + behind, 6, d, device="cuda").to(dtype)
 
         def put(cu, ids):
-            before, qo = c.k.clone(), torch.full((6, 2, d), 5.0, dtype=dtype, device="cuda")
+            before, qo = c.k.clone(), torch.full((6 + behind, 2, d), 5.0, dtype=dtype, device="cuda")
             c.append(0, x[:, :2], x[:, 2:4], x[:, 4:], ints(cu), ints(ids), q_out=qo)
             moved = (torch.nan_to_num(c.k, 9.0) != torch.nan_to_num(before, 9.0)).any(-1).any(2)[0]
             return qo, int(moved.sum())
@@ -799,6 +847,43 @@ def test_graphs_and_streams():
                 gg.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_chunks_in_a_graph(dtype):
+    """A mixed batch captured once and replayed while lengths, ids and the
+    batch itself change: two graphs of it, beside an eager call."""
+    hq, hk, d = 8, 2, 64
+    lens = [700, 90, 1500, 40]
+    c, ks, vs = filled(dtype, hk, d, 16, lens)
+    q = torch.randn(220, hq, d, device="cuda").to(dtype)
+    cu, ids = ints([0, 150, 151, 199, 220]), ints([0, 1, 2, 3])
+    eager = c.attention(0, q, cu, ids).clone()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c.attention(0, q, cu, ids))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        again = c.attention(0, q, cu, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager) and torch.equal(again, eager)
+    cu.copy_(ints([0, 1, 1, 180, 200]))
+    ids.copy_(ints([3, 0, 2, 0]))
+    c.seq_len[0] = 555
+    outs[0].fill_(3.0)
+    graphs[0].replay()
+    short = [k[:, :555] if s == 0 else k for s, k in enumerate(ks)], [v[:, :555] if s == 0 else v for s, v in enumerate(vs)]
+    want, tol = expected(q[:200], *short, [3, 0, 2, 0], [1, 0, 179, 20], 1 / math.sqrt(d), True, 0)
+    close(outs[0][:200], want, tol)
+    assert (outs[0][200:] == 3).all()
     c.check()
 
 
