@@ -232,7 +232,8 @@ int oc_sdpa(const float *q, const float *k, const float *v, float *o, int seq_le
  * attention calls alone may overlap.  Contents of device arrays (ids, offsets,
  * lengths) cannot be checked by the host: a kernel that meets a bad one sets
  * a bit of *status and stays inside the arrays.  extend, fork and copy_pages
- * then change nothing at all; the others skip the entry. */
+ * then change nothing at all; the others skip the entry.  (A page table that
+ * the caller has broken: fork passes a bad page number on, and reports it.) */
 #define OC_KV_F32 0
 #define OC_KV_F16 1
 #define OC_KV_BF16 2
@@ -298,10 +299,10 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * sees keys j < seq_len with j <= p when causal and j > p - window when
  * window > 0; a row that sees none gives 0, and what a row does not see has
  * no part in it, whatever it holds.  f32 accumulation and softmax statistics.
- * Sequences of up to 32 query rows per kv head (decode steps) are bound by the
+ * Sequences of few query rows per kv head (decode steps) are bound by the
  * cache's bytes and run on warp-level matrix instructions (f32: CUDA cores);
- * longer chunks with head_dim 64 or 128 and 16-byte-aligned rows run on the
- * tcgen05 tensor cores, f32 as pairs of f16 terms.
+ * more rows (over 16, f32 8) with head_dim 64 or 128 and 16-byte-aligned rows
+ * run on the tcgen05 tensor cores, f32 as pairs of f16 terms.
  * workspace: oc_kv_attention_workspace_size bytes, for partial results of
  * long sequences that several blocks share; calls that may overlap need one
  * each. */

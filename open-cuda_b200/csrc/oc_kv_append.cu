@@ -398,9 +398,11 @@ static int launch_append(KvAppend a, int interleaved, cudaStream_t s) {
                    quad(a.c.v) && quad(a.qw) && quad(a.kw) && a.qs % 4 == 0 && a.ks % 4 == 0 && a.vs % 4 == 0 && a.os % 4 == 0;
   const int lpr = !vec ? 32 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
   const int step = kAppendThreads / lpr, steps = (rows + step - 1) / step;
-  // few tokens: a token's rows over several CTAs, a step of them each (one
-  // token of 36 heads: 3 CTAs, 3.1 us; a warp for it: 6); many: a warp a token
-  const bool spread = (int64_t)a.bt.total * steps <= 4 * (int64_t)std::max(1, sm_count());
+  // few tokens: a token's rows over several CTAs, a step of them each; many: a
+  // warp a token.  Measured, 48 heads of 128 in f16, the first against the
+  // second: one token 2.5 us : 8.4, 64 tokens 3.0 : 10.2, 512 5.7 : 10.6,
+  // 1024 9.1 : 10.8, 1536 12.6 : 12.5, 4096 32 : 22 (three CTAs a token)
+  const bool spread = (int64_t)a.bt.total * steps <= 20 * (int64_t)std::max(1, sm_count());
   a.rows_per_cta = spread ? step : rows;
   const dim3 block(kAppendThreads);
   auto go = [&](auto kern, dim3 grid) {
@@ -444,6 +446,7 @@ extern "C" int oc_kv_append(const oc_kv_cache* cache, int layer, int tokens, int
   if (tokens == 0 || n == 0) return OC_OK;
   OC_REQUIRE(k && v && (q_heads == 0 || (q && q_out)), "kv_append: NULL pointer");
   OC_REQUIRE(n <= c.max_seqs, "kv_append: more entries than sequences");
+  OC_REQUIRE(((int64_t)q_heads + 2 * (int64_t)c.hk) * c.d <= INT_MAX, "kv_append: too many heads");
   const int64_t kd = (int64_t)c.hk * c.d, qd = (int64_t)q_heads * c.d;
   OC_REQUIRE(k_stride >= kd && v_stride >= kd && (q_heads == 0 || (q_stride >= qd && q_out_stride >= qd)),
              "kv_append: a token stride is shorter than its heads");

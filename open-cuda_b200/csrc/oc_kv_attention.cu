@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, KvParts parts, 
         }
         o = sum == 0.0f ? 0.0f : o / sum;
         out[threadIdx.x] = kv_from<T>(o);
-        bad = !isfinite(o);
+        bad = kv_lost<T>(o);
       }
       bad = __syncthreads_or(bad) && warp == 0;
     } else {
@@ -149,13 +149,14 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(KvAttn a, KvParts parts, 
           if (x < d) {
             const float o = l == 0.0f ? 0.0f : f[e] / l;
             out[x] = kv_from<T>(o);
-            bad |= !isfinite(o);
+            bad |= kv_lost<T>(o);
           }
         }
       }
       bad = __any_sync(0xffffffffu, bad);
+      __syncwarp();  // the row is written again, by other lanes
     }
-    // (oc_kv_mma.cuh) a row that is not finite is computed from the definition
+    // (oc_kv_rows.cuh) a row that was lost is computed from the definition
     if (bad) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
     if constexpr (R == 1) __syncthreads();
   }
@@ -229,10 +230,14 @@ static KvLaunch mma_launch(int d, int rows) {
 // Rows of the pools are whole, aligned 16-byte chunks.
 static bool vector_rows(const KvView& c, size_t esize) { return c.d * esize % 16 == 0 && aligned16(c.k) && aligned16(c.v); }
 
-// Query rows of a sequence's kv head up to which the warp-level kernel takes
-// it where both can: above, its 16- and 32-row items read the keys again and
-// again; below, 128-row tiles are mostly empty.
-constexpr int kFewRows = 32;
+// Query rows of a sequence's kv head up to which the few-row kernels take it
+// where both can.  Measured, 128-row tiles against them: f16, 16 sequences of
+// 4096 keys and heads of 128, 16 rows 103 us : 87, 28 rows 103 : 114, 64 rows
+// 106 : 179; one sequence of 16000, 16 rows 48 : 32, 28 rows 50 : 56.  f32, 16
+// of 4000 and heads of 64, 8 rows 245 : 238, 16 rows 257 : 453; one sequence,
+// 8 rows 36 : 36, 16 rows 38 : 48.
+template <typename T>
+constexpr int kFewRows = sizeof(T) == 4 ? 8 : 16;
 
 // The launches of a call, each over its class of sequences.  one_each: every
 // sequence has one new token; qvec: rows of q are whole 16-byte chunks.
@@ -241,34 +246,40 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
   const int group = q_heads / c.hk;
   const int most = one_each ? group : tokens * group;                 // rows that a sequence can have
   const int likely = tokens <= n ? std::min(group, most) : most;      // and those to choose a shape by
-  const bool tile = (c.d == 64 || c.d == 128) && tokens > n && most > kFewRows && is_sm100() &&
-                    (sizeof(T) == 4 || (qvec && vector_rows(c, sizeof(T))));
-  if constexpr (sizeof(T) == 4) {
-    out[0] = scalar_launch<T>(c.d, tile ? kFewRows : likely);
-    if (tile) {
-      auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>, 2); };
-      out[1] = c.d == 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
-    }
+  constexpr int few = kFewRows<T>;
+  const bool tile = (c.d == 64 || c.d == 128) && likely > few && is_sm100() && (sizeof(T) == 4 || (qvec && vector_rows(c, sizeof(T))));
+  int count = 0;
+  if (!tile) {
+    if constexpr (sizeof(T) == 4)
+      out[count++] = scalar_launch<T>(c.d, likely);
+    else
+      out[count++] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, likely) : scalar_launch<T>(c.d, likely);
   } else {
-    // beside chunks that go to the tiles the few rows are mostly single tokens'
-    // (16 rows an item), unless the whole batch is of a few tokens each
-    const int64_t mean = (int64_t)tokens * group / std::max(1, n);
-    const int few = mean <= 2 * kFewRows ? kFewRows : std::min(kFewRows, group);
-    out[0] = vector_rows(c, sizeof(T)) ? mma_launch<T>(c.d, tile ? few : likely) : scalar_launch<T>(c.d, likely);
-    if (tile) {
+    if (group <= few) {  // else a single token has more rows
+      if constexpr (sizeof(T) == 4) {
+        // beside long chunks the few rows are mostly single tokens', unless the
+        // whole batch is of a few tokens each
+        const int64_t mean = (int64_t)tokens * group / std::max(1, n);
+        out[count] = scalar_launch<T>(c.d, mean <= 4 * few ? few : group);
+      } else {
+        out[count] = mma_launch<T>(c.d, few);
+      }
+      out[count++].rows_max = few;
+    }
+    if constexpr (sizeof(T) == 4) {
+      auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>, 2); };
+      out[count] = c.d == 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
+    } else {
       auto go = [](auto k) {
         KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
         l.tile = kv_tile_kernel<decltype(k)>;
         return l;
       };
-      out[1] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
+      out[count] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
     }
+    out[count].rows_min = count ? few : 0;
+    out[count++].one_per_sm = true;
   }
-  if (tile) {
-    out[0].rows_max = out[1].rows_min = kFewRows;
-    out[1].one_per_sm = true;
-  }
-  const int count = tile ? 2 : 1;
   for (int i = 0; i < count; ++i) {
     const void* fn = out[i].fn();
     smem_attr_once(fn, out[i].smem);  // before the occupancy is asked for

@@ -1,15 +1,16 @@
-// oc_kv_mma.cuh -- attention over the paged cache for up to 32 query rows of
-// an item, f16 and bf16: decode steps and short chunks.
+// oc_kv_mma.cuh -- attention over the paged cache in items of 16 or 32 query
+// rows, f16 and bf16: decode steps, and chunks of head_dims that the tcgen05
+// tiles do not take.
 //
 // Bound: the cache's bytes (a decode step of 8 rows does 32 flops per element
 // read).  On the CUDA cores 8 rows cost more issue slots than the memory
 // leaves (0.1 of the copy rate measured, 3.7 ms for 64 sequences of 2 to 15 k
-// keys, 32 heads of 128 over 8; here 385 us = 5.86 TB/s, 0.91), so the products run on warp-level
-// matrix instructions, whose 16 rows a decode step's query heads of one kv
-// head fill in part; tcgen05 tiles of 128 rows would be mostly empty and
-// would put a block-wide hand-over behind every tile.  A warp works alone:
-// its own 16-key tiles, its own cp.async ring, its own softmax; only the end
-// of an item is a meeting.
+// keys, 32 heads of 128 over 8; here 385 us = 5.86 TB/s, 0.91), so the
+// products run on warp-level matrix instructions, whose 16 rows a decode
+// step's query heads of one kv head fill in part; tcgen05 tiles of 128 rows
+// would be mostly empty and would put a block-wide hand-over behind every
+// tile.  A warp works alone: its own 16-key tiles, its own cp.async ring, its
+// own softmax; only the end of an item is a meeting.
 //   S = Q K^T   16 rows x 16 keys: two m16n8k16 per 16 features (K read with
 //               ldmatrix: its rows are the columns of the second operand)
 //   O += P V    two m16n8k16 per 16 features (V read with ldmatrix.trans),
@@ -57,47 +58,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// One row of one query head from the definition, by one warp: for rows whose
-// result is not finite.  Reads only keys that the row sees.
-template <typename T>
-__device__ __noinline__ void kv_row_exact(const KvAttn& a, const KvSeq& s, int h, int row) {
-  const KvView& c = a.c;
-  const int lane = threadIdx.x & 31, d = c.d, g = a.p.group;
-  const int64_t token = s.q0 + row / g, head = (int64_t)(h * g + row % g) * d;
-  const T* q = static_cast<const T*>(a.q) + token * a.qs + head;
-  const T* kb = static_cast<const T*>(c.k) + a.layer_off;
-  const T* vb = static_cast<const T*>(c.v) + a.layer_off;
-  int lo, hi;
-  plan_row_range(a.p, s, row, lo, hi);
-  float x[8], o[8] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = lane + 32 * i < d ? kv_f32(q[lane + 32 * i]) : 0.0f;
-  for (int key = lo; key < hi; ++key) {
-    const int64_t off = kv_row_off(a, s.s, h, key, lo, hi);
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < d && off >= 0) dot = fmaf(x[i], kv_f32(kb[off + lane + 32 * i]), dot);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-    dot *= a.scale2;
-    const float mn = fmaxf(m, dot), base = mn == -INFINITY ? 0.0f : mn;
-    const float corr = exp2f(m - base), p = exp2f(dot - base);
-    m = mn;
-    l = fmaf(l, corr, p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < d) {
-        const float v = off >= 0 ? kv_f32(vb[off + lane + 32 * i]) : 0.0f;
-        o[i] = fmaf(p, v, corr == 1.0f ? o[i] : o[i] * corr);
-      }
-  }
-  T* out = static_cast<T*>(a.out) + token * a.os + head;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < d) out[lane + 32 * i] = kv_from<T>(l == 0.0f ? 0.0f : o[i] / l);
 }
 
 template <typename T_, int DP_, int MT_>
@@ -360,7 +320,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
         if (e < d) {
           const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
           os.x *= inv, os.y *= inv;
-          if (!isfinite(os.x) || !isfinite(os.y)) bad |= 1u << r;
+          if (kv_lost<T>(os.x) || kv_lost<T>(os.y)) bad |= 1u << r;
           T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.os + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e;
           if (a.ovec) {
             *reinterpret_cast<uint32_t*>(out) = kv_pack2<T>(os.x, os.y);

@@ -10,7 +10,11 @@
 // half warp keeps a softmax of its own (running maximum and sum, log2 units),
 // four keys at a time.  The halves and warps meet in shared memory at the end
 // of an item.  A key that a row does not see is left out by a predicate, not
-// by a zero weight, so what it holds cannot reach the row.
+// by a zero weight, so what it holds cannot reach the row.  Weights are kept
+// at 2^-24 or less (the running maximum is held 24 higher), so that the sums
+// of 2^24 values near the type's largest stay finite: a second look at lost
+// rows, as the other kernels take it, would cost this one its registers (168
+// -> 238 a thread, 14 % slower).
 #pragma once
 #include "oc_kv_plan.cuh"
 
@@ -48,6 +52,61 @@ __device__ __forceinline__ int64_t kv_row_off(const KvAttn& a, int seq, int h, i
     return -1;
   }
   return ((((int64_t)page * c.hk + h) << c.ps_shift) + (key & ((1 << c.ps_shift) - 1))) * c.d;
+}
+
+// A result that is not finite, or that rounding to T would make infinite
+// (half a step above T's largest value).
+template <typename T>
+__device__ __forceinline__ bool kv_lost(float y) {
+  if constexpr (std::is_same<T, __half>::value) return !(fabsf(y) < 65520.0f);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return !(fabsf(y) < __uint_as_float(0x7f7f8000u));
+  return !isfinite(y);
+}
+
+// One row of one query head from the definition, by one warp: for rows whose
+// result was lost.  Reads only keys that the row sees; the weights are
+// divided by their sum before they meet the values, so values near the type's
+// largest do not overflow (the fast kernels divide at the end).
+template <typename T>
+__device__ __noinline__ void kv_row_exact(const KvAttn& a, const KvSeq& s, int h, int row) {
+  const KvView& c = a.c;
+  const int lane = threadIdx.x & 31, d = c.d, g = a.p.group;
+  const int64_t token = s.q0 + row / g, head = (int64_t)(h * g + row % g) * d;
+  const T* q = static_cast<const T*>(a.q) + token * a.qs + head;
+  const T* kb = static_cast<const T*>(c.k) + a.layer_off;
+  const T* vb = static_cast<const T*>(c.v) + a.layer_off;
+  int lo, hi;
+  plan_row_range(a.p, s, row, lo, hi);
+  float x[8], o[8] = {}, m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = lane + 32 * i < d ? kv_f32(q[lane + 32 * i]) : 0.0f;
+  auto score = [&](int64_t off) {
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < d && off >= 0) dot = fmaf(x[i], kv_f32(kb[off + lane + 32 * i]), dot);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+    return dot * a.scale2;
+  };
+  for (int key = lo; key < hi; ++key) {
+    const float dot = score(kv_row_off(a, s.s, h, key, lo, hi));
+    const float mn = fmaxf(m, dot), base = mn == -INFINITY ? 0.0f : mn;
+    l = fmaf(l, exp2f(m - base), exp2f(dot - base));
+    m = mn;
+  }
+  const float base = m == -INFINITY ? 0.0f : m;
+  for (int key = lo; key < hi; ++key) {
+    const int64_t off = kv_row_off(a, s.s, h, key, lo, hi);
+    const float p = exp2f(score(off) - base), w = l == 0.0f ? 0.0f : p / l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < d) o[i] = fmaf(w, off >= 0 ? kv_f32(vb[off + lane + 32 * i]) : 0.0f, o[i]);
+  }
+  T* out = static_cast<T*>(a.out) + token * a.os + head;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (lane + 32 * i < d) out[lane + 32 * i] = kv_from<T>(l == 0.0f ? 0.0f : o[i]);
 }
 
 // Requests the 16 rows whose offsets lanes 0..15 (and 16..31 again) hold.
@@ -223,7 +282,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           const float mx = fmaxf(fmaxf(s[0][r], s[1][r]), fmaxf(s[2][r], s[3][r]));
-          const float mn = fmaxf(m[r], mx), base = mn == -INFINITY ? 0.0f : mn;
+          const float mn = fmaxf(m[r], mx + 24.0f), base = mn == -INFINITY ? 0.0f : mn;
           const float corr = exp2f(m[r] - base);
           m[r] = mn;
           float add = 0.0f;

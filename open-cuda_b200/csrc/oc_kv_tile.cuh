@@ -15,11 +15,11 @@
 // the chain of a sub-tile (scores out of tensor memory 420 cycles, maximum
 // 370, exponentials 1500, then its two products): 3900 cycles a tile by a
 // clock record.  Measured: chunks of 1.9 to 2 k tokens over 14 to 16 k keys,
-// 32 heads of 128 over 8, 930 to 1010 us = 0.9 to 0.98 PFLOP/s.  Not kept, all slower there:
-// two threads a row (16 softmax warps, 96 registers: 1120 us), exponentials
-// in part as polynomials on the multiply-add pipe (1060 to 1200), items of 128
-// rows whose tiles two softmax groups take in turn (1215: twice the keys'
-// traffic).  O stays in tensor memory and is rescaled only when a row's
+// 32 heads of 128 over 8, 930 to 1010 us = 0.9 to 0.98 PFLOP/s.  Not kept, all
+// slower there: two threads a row (16 softmax warps, 96 registers: 1120 us),
+// exponentials in part as polynomials on the multiply-add pipe (1060 to 1200),
+// items of 128 rows whose tiles two softmax groups take in turn (1215: twice
+// the keys' traffic).  O stays in tensor memory and is rescaled only when a row's
 // maximum grows by more than 2^8 since the last time (weights up to 2^8 lose
 // nothing in either type): after the first tiles that is rare, so the softmax
 // almost never waits for the accumulator.
@@ -40,9 +40,9 @@
 //
 // P is rounded once to the operands' type (bf16: 2^-9 at most, as much as the
 // result's own rounding); sums and maxima are f32, the sum of P is taken
-// before the rounding.  Rows that are not finite are computed again from the
-// definition (kv_row_exact): a zero weight does not hide a NaN or an infinity
-// of a key that the row does not see.
+// before the rounding.  Rows that are not finite, or would not be once rounded,
+// are computed again from the definition (kv_row_exact): a zero weight does
+// not hide a NaN or an infinity of a key that the row does not see.
 #pragma once
 #include "oc_flash_tc.cuh"
 #include "oc_kv_mma.cuh"
@@ -197,7 +197,8 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs<KvTileBars>
 }
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+__global__ void __launch_bounds__(K::THREADS, 1)
+    kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const __grid_constant__ CUtensorMap mq, int box, int qbox) {
   using T = typename K::T;
   using R = KvTileRows<K>;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile_kernel(KvAttn a, const 
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const float y0 = __uint_as_float(o[e + 2 * k]) * inv, y1 = __uint_as_float(o[e + 2 * k + 1]) * inv;
-                  bad |= !isfinite(y0) || !isfinite(y1);
+                  bad |= kv_lost<T>(y0) || kv_lost<T>(y1);
                   p[k] = kv_pack2<T>(y0, y1);
                 }
                 if (a.ovec16) {

@@ -18,7 +18,8 @@ can be captured into a CUDA graph.
 `seqs`, `counts`, `cu`, ... are int32 CUDA tensors: entry b of a batch is
 sequence seqs[b] (seqs None: b) with new tokens cu[b] .. cu[b + 1] - 1 (cu
 None: one token each).  Calls on one cache are ordered by the caller (one
-stream, or events); attention alone may run on several streams at once.
+stream, or events); attention alone may run on several streams at once
+(threads that use one stream take turns: its calls share a workspace).
 """
 from __future__ import annotations
 
@@ -142,6 +143,9 @@ class KVCache:
         """Scratch of one attention call: eager calls of one stream run one
         after another and share a buffer; a captured call gets its own, which
         its graph keeps."""
+        if self._current_device() != self._index:
+            with self._torch.cuda.device(self._index):
+                return self._workspace(need)
         stream = self._raw_stream(self._index)
         if self._torch.cuda.is_current_stream_capturing():
             return self._new_bytes(need)
@@ -191,6 +195,7 @@ class KVCache:
         """Waits for the cache's device and raises ValueError if a call since
         the last check met something it refuses, OcError if a wait inside a
         kernel expired."""
+        self._torch.cuda.synchronize(self.device)  # calls of every stream
         bits = int(self.status.item())
         expired = oc.ci(0)
         with self._torch.cuda.device(self._index):
@@ -208,8 +213,8 @@ class KVCache:
         """Norms (q_weight, k_weight [head_dim]) and rotation (inv_freq
         [rot_dim / 2] f32) of the new tokens' queries [tokens, q_heads,
         head_dim] and keys [tokens, kv_heads, head_dim], keys and values
-        written to their pages.  Returns the queries (q_out, or a new tensor;
-        q None: keys and values alone)."""
+        written to their pages.  Returns the queries (q_out, or a new tensor,
+        unset behind the last sequence; q None: keys and values alone)."""
         tokens, d = k.shape[0], self.head_dim
         ks, vs = self._rows(k, tokens, self.kv_heads, "k"), self._rows(v, tokens, self.kv_heads, "v")
         n, cp, sp = self._batch(tokens, cu, seqs)
@@ -247,7 +252,8 @@ class KVCache:
         """softmax(scale q . K^T) V of the new tokens' queries [tokens,
         q_heads, head_dim] over their sequences' pages (scale None: 1 /
         sqrt(head_dim)); causal, and the last `window` keys alone when window
-        > 0.  Rows of `out` behind the last sequence stay as they are."""
+        > 0.  Rows of `out` behind the last sequence stay as they are (in a new
+        tensor: unset)."""
         if q.dim() != 3:
             raise ValueError(f"kv_cache: q is [tokens, q_heads, {self.head_dim}], got {tuple(q.shape)}")
         tokens, heads, d = q.shape

@@ -224,6 +224,24 @@ def test_unaligned_queries_and_pools(dtype):
     close(attend(moved, q, [0, 1], [1, 3]), want, tol)
 
 
+@pytest.mark.parametrize("dtype, big", [(F32, 3e38), (F16, 65504.0), (BF16, torch.finfo(BF16).max)])
+@pytest.mark.parametrize("hq, hk, d", [(8, 2, 64), (4, 2, 128), (4, 2, 80), (2, 2, 256), (3, 1, 17)])
+@pytest.mark.parametrize("lens, new", [([9, 40], [1, 1]), ([3000], [1]), ([300, 1500], [20, 100]), ([2100], [260])])
+def test_values_near_the_largest(dtype, big, hq, hk, d, lens, new):
+    """Sums of weights times values overflow, the outputs do not: in whole
+    items, joined ones and chunks.  Every value of a feature is plus or minus
+    `big`, and so is the output (weights sum to one)."""
+    c, ks, vs = filled(dtype, hk, d, 16, lens, seed=d)
+    sign = torch.where(torch.arange(d, device="cuda") % 3 == 0, -1.0, 1.0).double()
+    c.v.copy_((sign * big).to(dtype).expand(c.v.shape))
+    q = torch.randn(sum(new), hq, d, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(dtype)
+    o = attend(c, q, range(len(lens)), new)
+    want, tol = expected(q, ks, [x.copy_((sign * big).to(dtype).expand(x.shape)) for x in vs], range(len(lens)), new, 1 / math.sqrt(d), True, 0)
+    assert torch.isfinite(o).all()
+    close(o, want, tol)
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 80, 128])
 @pytest.mark.parametrize("new", [[1, 1], [1, 90], [90, 200]])

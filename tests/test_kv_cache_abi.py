@@ -59,7 +59,7 @@ def append(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=512,
 @pytest.mark.parametrize("args, word", [
     (dict(layer=2), "layer"), (dict(n=3), "one token"), (dict(rot=3, inv=0x9000), "even"), (dict(rot=66, inv=0x9000), "rot_dim"),
     (dict(rot=64), "inv_freq"), (dict(k=None), "NULL"), (dict(qo=None), "NULL"), (dict(ks=255), "stride"), (dict(qs=511), "stride"),
-    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"),
+    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"), (dict(heads=1 << 26, qs=1 << 33, qos=1 << 33), "too many heads"),
 ])
 def test_append_refusals(args, word):
     assert append(**args) == oc.OC_ERR_INVALID_VALUE
