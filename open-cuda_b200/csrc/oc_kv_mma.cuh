@@ -80,7 +80,7 @@ struct KvMma {
 };
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(KvAttn a) {
+__global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __grid_constant__ KvAttn a) {
   using T = typename K::T;
   using L = typename K::L;
   constexpr int DP = K::DP, MT = K::MT, NS = K::NS, KS = DP / 16, ROWS = K::ROWS, OS = K::OS;

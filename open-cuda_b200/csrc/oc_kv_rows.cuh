@@ -167,7 +167,7 @@ struct KvRows {
 };
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(KvAttn a) {
+__global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_constant__ KvAttn a) {
   using T = typename K::T;
   using L = typename K::L;
   constexpr int ROWS = K::ROWS, F = K::F, NV = K::NV, VN = K::VN, NS = K::NS, DP = K::DP;

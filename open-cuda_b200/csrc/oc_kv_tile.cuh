@@ -198,7 +198,7 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs<KvTileBars>
 
 template <typename K>
 __global__ void __launch_bounds__(K::THREADS, 1)
-    kv_tile_kernel(KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+    kv_tile_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const __grid_constant__ CUtensorMap mq, int box, int qbox) {
   using T = typename K::T;
   using R = KvTileRows<K>;

@@ -139,7 +139,7 @@ __device__ __forceinline__ void kv_mask_chunk(uint32_t (&r)[32], int from, int t
 }
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(KvAttn a) {
+__global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_constant__ KvAttn a) {
   constexpr int D = K::D;
   extern __shared__ uint8_t raw[];
   __shared__ KvPlanShared plan;
