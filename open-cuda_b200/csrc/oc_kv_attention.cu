@@ -29,7 +29,7 @@ struct KvParts {
 // would mostly be launched to find nothing (2065 CTAs, 8 us, at 296 x 7).
 // DP: features of a row, 128 or 256.
 template <typename T, int R, int DP>
-__global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, KvParts parts, int dp) {
+__global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts, int dp) {
   constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
   __shared__ float part[R == 1 ? WARPS : 1][DP], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
   __shared__ unsigned short list[2][kMostCtas];

@@ -68,7 +68,7 @@ __device__ __forceinline__ bool kv_lost(float y) {
 // divided by their sum before they meet the values, so values near the type's
 // largest do not overflow (the fast kernels divide at the end).
 template <typename T>
-__device__ __noinline__ void kv_row_exact(const KvAttn& a, const KvSeq& s, int h, int row) {
+__device__ __noinline__ void kv_row_exact(const KvAttn& a, KvSeq s, int h, int row) {
   const KvView& c = a.c;
   const int lane = threadIdx.x & 31, d = c.d, g = a.p.group;
   const int64_t token = s.q0 + row / g, head = (int64_t)(h * g + row % g) * d;
