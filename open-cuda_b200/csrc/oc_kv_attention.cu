@@ -33,31 +33,45 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
   constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
   __shared__ float part[R == 1 ? WARPS : 1][DP], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
   __shared__ unsigned short list[2][kMostCtas];
-  __shared__ int wcount[WARPS];
+  __shared__ int wcount[2][WARPS];
   const KvView& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = c.d;
   pdl_wait();
-  int found[2] = {0, 0};
+  // each thread looks at every 256th CTA's cut, all requested at once; the
+  // order of the list does not matter
+  constexpr int ROUNDS = kMostCtas / 256;
+  uint32_t mine[2] = {0, 0};
+  int before[2], found[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (k >= parts.count) break;
-    const KvCut* cuts = reinterpret_cast<const KvCut*>(parts.of[k].ws);
-    for (int i0 = 0; i0 < parts.of[k].ctas; i0 += 256) {
-      const int i = i0 + threadIdx.x;
-      const bool there = i < parts.of[k].ctas && cuts[i].pieces > 0;
-      const uint32_t votes = __ballot_sync(0xffffffffu, there);
-      if (lane == 0) wcount[warp] = __popc(votes);
-      __syncthreads();
-      int at = found[k];
+    if (k < parts.count) {
+      const KvCut* cuts = reinterpret_cast<const KvCut*>(parts.of[k].ws);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) at += wcount[w];
-        found[k] += wcount[w];
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int cta = i * 256 + threadIdx.x;
+        if (cta < parts.of[k].ctas && cuts[cta].pieces > 0) mine[k] |= 1u << i;
       }
-      if (there) list[k][at + __popc(votes & ((1u << lane) - 1))] = (unsigned short)i;
-      __syncthreads();
     }
+    before[k] = __popc(mine[k]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before[k], o);
+      if (lane >= o) before[k] += y;
+    }
+    if (lane == 31) wcount[k][warp] = before[k];
+    before[k] -= __popc(mine[k]);
   }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before[k] += wcount[k][w];
+      found[k] += wcount[k][w];
+    }
+    for (uint32_t todo = mine[k]; todo; todo &= todo - 1) list[k][before[k]++] = (unsigned short)((__ffs(todo) - 1) * 256 + threadIdx.x);
+  }
+  __syncthreads();
   const int tasks0 = found[0] * parts.of[0].groups, tasks = tasks0 + found[1] * parts.of[1].groups;
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
     const bool second = task >= tasks0;

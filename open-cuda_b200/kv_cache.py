@@ -80,6 +80,7 @@ class KVCache:
         lib = oc.lib()
         self._torch, self._index, self._int32, self._f32 = torch, k.device.index, torch.int32, torch.float32
         self._current_device, self._raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        self._capturing, self._empty_like, self._scale = torch.cuda.is_current_stream_capturing, torch.empty_like, 1.0 / math.sqrt(dim)
         self._append, self._attention, self._extend, self._fork = lib.oc_kv_append, lib.oc_kv_attention, lib.oc_kv_extend, lib.oc_kv_fork
         self._free, self._compact, self._copy = lib.oc_kv_free, lib.oc_kv_compact, lib.oc_kv_copy_pages
         self._ws_bytes, self._workspaces = {}, {}
@@ -138,21 +139,6 @@ class KVCache:
                 rc = fn(self._p, *args, self._raw_stream(index))
         if rc:
             oc.check(rc)
-
-    def _workspace(self, need):
-        """Scratch of one attention call: eager calls of one stream run one
-        after another and share a buffer; a captured call gets its own, which
-        its graph keeps."""
-        if self._current_device() != self._index:
-            with self._torch.cuda.device(self._index):
-                return self._workspace(need)
-        stream = self._raw_stream(self._index)
-        if self._torch.cuda.is_current_stream_capturing():
-            return self._new_bytes(need)
-        ws = self._workspaces.get(stream)
-        if ws is None or ws.numel() < need:
-            ws = self._workspaces[stream] = self._new_bytes(need)
-        return ws
 
     def _new_bytes(self, need):
         return self._torch.empty(need, dtype=self._torch.uint8, device=self.device)
@@ -215,6 +201,10 @@ class KVCache:
         head_dim] and keys [tokens, kv_heads, head_dim], keys and values
         written to their pages.  Returns the queries (q_out, or a new tensor,
         unset behind the last sequence; q None: keys and values alone)."""
+        index = self._index
+        if self._current_device() != index:
+            with self._torch.cuda.device(index):
+                return self.append(layer, q, k, v, cu, seqs, q_weight, k_weight, eps, inv_freq, interleaved, q_out)
         tokens, d = k.shape[0], self.head_dim
         ks, vs = self._rows(k, tokens, self.kv_heads, "k"), self._rows(v, tokens, self.kv_heads, "v")
         n, cp, sp = self._batch(tokens, cu, seqs)
@@ -224,7 +214,7 @@ class KVCache:
             heads = q.shape[1]
             qs = self._rows(q, tokens, heads, "q")
             if q_out is None:
-                q_out = q.new_empty(q.shape)
+                q_out = self._empty_like(q)  # contiguous: the heads of q's tokens are
                 os_ = heads * d
             else:
                 os_ = self._rows(q_out, tokens, heads, "q_out")
@@ -239,8 +229,10 @@ class KVCache:
             if inv_freq.dim() != 1 or inv_freq.dtype != self._f32 or not inv_freq.is_contiguous() or inv_freq.device != self.device:
                 raise ValueError(f"kv_cache: inv_freq is a float32 vector on {self.device}")
             rot, ip = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-        self._call(self._append, layer, tokens, n, cp, sp, heads, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, op, os_, qw, kw, eps, ip, rot,
-                   1 if interleaved else 0)
+        rc = self._append(self._p, layer, tokens, n, cp, sp, heads, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, op, os_, qw, kw, eps, ip, rot,
+                          1 if interleaved else 0, self._raw_stream(index))
+        if rc:
+            oc.check(rc)
         return q_out
 
     def _weight(self, w):
@@ -254,20 +246,34 @@ class KVCache:
         sqrt(head_dim)); causal, and the last `window` keys alone when window
         > 0.  Rows of `out` behind the last sequence stay as they are (in a new
         tensor: unset)."""
+        index = self._index
+        if self._current_device() != index:
+            with self._torch.cuda.device(index):
+                return self.attention(layer, q, cu, seqs, scale, causal, window, out)
         if q.dim() != 3:
             raise ValueError(f"kv_cache: q is [tokens, q_heads, {self.head_dim}], got {tuple(q.shape)}")
         tokens, heads, d = q.shape
         qs = self._rows(q, tokens, heads, "q")
         n, cp, sp = self._batch(tokens, cu, seqs)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = self._empty_like(q)  # contiguous: the heads of q's tokens are
             os_ = heads * d
         else:
             os_ = self._rows(out, tokens, heads, "out")
         need = self._ws_bytes.get((tokens, n, heads)) or self._workspace_size(tokens, n, heads)
-        ws = self._workspace(need)
-        self._call(self._attention, layer, tokens, n, cp, sp, heads, q.data_ptr(), qs, out.data_ptr(), os_,
-                   1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, window, ws.data_ptr(), need)
+        stream = self._raw_stream(index)
+        # eager calls of one stream run one after another and share a scratch
+        # buffer; a captured call gets its own, which its graph keeps
+        if self._capturing():
+            ws = self._new_bytes(need)
+        else:
+            ws = self._workspaces.get(stream)
+            if ws is None or ws.numel() < need:
+                ws = self._workspaces[stream] = self._new_bytes(need)
+        rc = self._attention(self._p, layer, tokens, n, cp, sp, heads, q.data_ptr(), qs, out.data_ptr(), os_,
+                             self._scale if scale is None else scale, 1 if causal else 0, window, ws.data_ptr(), need, stream)
+        if rc:
+            oc.check(rc)
         return out
 
     def _workspace_size(self, tokens, n, heads):
