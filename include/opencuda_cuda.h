@@ -301,8 +301,8 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * no part in it, whatever it holds.  f32 accumulation and softmax statistics.
  * Sequences of few query rows per kv head (decode steps) are bound by the
  * cache's bytes and run on warp-level matrix instructions (f32: CUDA cores);
- * more rows (over 16, f32 8) with head_dim 64 or 128 and 16-byte-aligned rows
- * run on the tcgen05 tensor cores, f32 as pairs of f16 terms.
+ * more rows (over 16, f32 8) of head_dim up to 128 run on the tcgen05 tensor
+ * cores, f32 as pairs of f16 terms (f16 and bf16: 16-byte-aligned rows).
  * workspace: oc_kv_attention_workspace_size bytes, for partial results of
  * long sequences that several blocks share; calls that may overlap need one
  * each. */

@@ -12,7 +12,7 @@ constexpr int kMostCtas = 2048;  // of an attention kernel's grid
 // The partial results of one launch.
 struct KvPart {
   float* ws;
-  int ctas, br, groups;  // groups: of R rows, that an item can have
+  int ctas, br, groups, dp;  // groups: of R rows, that an item can have; dp: floats of a row
 };
 struct KvParts {
   KvPart of[2];
@@ -29,7 +29,7 @@ struct KvParts {
 // would mostly be launched to find nothing (2065 CTAs, 8 us, at 296 x 7).
 // DP: features of a row, 128 or 256.
 template <typename T, int R, int DP>
-__global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts, int dp) {
+__global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts) {
   constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
   __shared__ float part[R == 1 ? WARPS : 1][DP], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
   __shared__ unsigned short list[2][kMostCtas];
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
     const bool second = task >= tasks0;
     const KvPart& pt = parts.of[second];
-    const int number = second ? task - tasks0 : task, br = pt.br;
+    const int number = second ? task - tasks0 : task, br = pt.br, dp = pt.dp;
     const int cta = list[second][number / pt.groups];
     const KvCut cut = reinterpret_cast<const KvCut*>(pt.ws)[cta];
     const int pieces = cut.pieces, r = (number % pt.groups) * R + warp / SPLIT;
@@ -261,7 +261,7 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
   const int most = one_each ? group : tokens * group;                 // rows that a sequence can have
   const int likely = tokens <= n ? std::min(group, most) : most;      // and those to choose a shape by
   constexpr int few = kFewRows<T>;
-  const bool tile = (c.d == 64 || c.d == 128) && likely > few && is_sm100() && (sizeof(T) == 4 || (qvec && vector_rows(c, sizeof(T))));
+  const bool tile = c.d <= 128 && likely > few && is_sm100() && (sizeof(T) == 4 || (qvec && vector_rows(c, sizeof(T))));
   int count = 0;
   if (!tile) {
     if constexpr (sizeof(T) == 4)
@@ -282,14 +282,14 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
     }
     if constexpr (sizeof(T) == 4) {
       auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>, 2); };
-      out[count] = c.d == 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
+      out[count] = c.d <= 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
     } else {
       auto go = [](auto k) {
         KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
         l.tile = kv_tile_kernel<decltype(k)>;
         return l;
       };
-      out[count] = c.d == 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
+      out[count] = c.d <= 64 ? go(KvTile<T, 64>()) : go(KvTile<T, 128>());
     }
     out[count].rows_min = count ? few : 0;
     out[count++].one_per_sm = true;
@@ -349,9 +349,9 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
           return rc;
       OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], m[2], box, qbox));
     }
-    parts.of[i] = KvPart{a.ws, l[i].ctas, l[i].br, 0};
+    parts.of[i] = KvPart{a.ws, l[i].ctas, l[i].br, 0, l[i].dp};
     a.ws += part_floats(l[i]);
-    dp = l[i].dp;
+    dp = std::max(dp, l[i].dp);
     rows = std::max(rows, l[i].merge_rows);
   }
   // the rows of one item that the joining kernel takes at a time: see there
@@ -365,7 +365,7 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
   if (tasks == 0) return OC_OK;  // one CTA: nothing is cut
   const int grid = (int)std::min<int64_t>(tasks, (few ? 4 : 8) * (int64_t)std::max(1, sm_count()));
   auto go = [&](auto kern) {
-    OC_CHECK_CUDA(launch_pdl_ex(kern, dim3(grid), dim3(256), 0, s, a, parts, dp));
+    OC_CHECK_CUDA(launch_pdl_ex(kern, dim3(grid), dim3(256), 0, s, a, parts));
     return OC_OK;
   };
   if (dp <= 128) return few ? go(kv_merge_kernel<T, 1, 128>) : go(kv_merge_kernel<T, 8, 128>);

@@ -5,7 +5,7 @@
 // Bound: the cache's bytes (a decode step of 8 rows does 32 flops per element
 // read).  On the CUDA cores 8 rows cost more issue slots than the memory
 // leaves (0.1 of the copy rate measured, 3.7 ms for 64 sequences of 2 to 15 k
-// keys, 32 heads of 128 over 8; here 385 us = 5.86 TB/s, 0.91), so the
+// keys, 32 heads of 128 over 8; here 374 us = 6.03 TB/s, 0.93), so the
 // products run on warp-level matrix instructions, whose 16 rows a decode
 // step's query heads of one kv head fill in part; tcgen05 tiles of 128 rows
 // would be mostly empty and would put a block-wide hand-over behind every

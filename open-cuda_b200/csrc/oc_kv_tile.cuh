@@ -1,5 +1,7 @@
 // oc_kv_tile.cuh -- attention over the paged cache for chunks of new tokens,
-// f16 and bf16, head_dim 64 and 128, on the tcgen05 tensor cores.
+// f16 and bf16, on the tcgen05 tensor cores.  D: head_dim, or 64 or 128 above
+// it with zeros behind (TMA fills them in; they cost the product with V, not
+// the scores).
 //
 // An item is 256 query rows (two sub-tiles of 128) of one kv head; it walks
 // tiles of 128 keys.  Per tile and sub-tile:
@@ -170,7 +172,7 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs<KvTileBars>
         if (lane == 0) mbar_arrive_expect_tx(&full[st], K::TILE);
         __syncwarp();
         if (lane < boxes) {
-          const int y = (int)(a.layer_off / K::D) + (int)((((int64_t)page * c.hk + it.h) << c.ps_shift) +
+          const int y = (int)(a.layer_off / c.d) + (int)((((int64_t)page * c.hk + it.h) << c.ps_shift) +
                                                           ((key0 + my_key) & ((1 << c.ps_shift) - 1)));
           tma_load_2d(dst + my_panel * K::PANEL + my_key * 128, map, my_panel * 64, y, &full[st]);
         }
@@ -181,7 +183,8 @@ __device__ __forceinline__ bool kv_tile_load(const KvAttn& a, KvJobs<KvTileBars>
 #pragma unroll 4
           for (int y = 0; y < 32; y += R::RPI) {
             const int64_t o = __shfl_sync(0xffffffffu, off, y + my_row);
-            cp_async16_zfill(dst + R::off(x + y + my_row, ch), pool + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+            const bool there = o >= 0 && ch * 8 < c.d;
+            cp_async16_zfill(dst + R::off(x + y + my_row, ch), pool + (there ? o + ch * 8 : 0), there);
           }
         }
         cp_async_commit();
@@ -271,6 +274,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
         const uint32_t q0 = smem_u32(sq) + sub * K::TILE, k0 = smem_u32(sk) + (tile & 1) * K::TILE;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
+          if (kk * 16 >= c.d) break;  // (zeros behind head_dim)
           const uint32_t off = (uint32_t)(kk >> 2) * K::PANEL + (uint32_t)(kk & 3) * 32;
           mma_f16(tmem + K::S_COL + sub * 128, desc_kmajor_sw128(q0 + off), desc_kmajor_sw128(k0 + off), idesc_s, kk != 0);
         }
@@ -369,12 +373,13 @@ __global__ void __launch_bounds__(K::THREADS, 1)
 #pragma unroll 1
         for (int x = 0; x < subs * 128; x += 32) {
           const int r = x + lane, rr = cur.it.r0 + r, token = plan_token(a.p, rr);  // zeros behind the last row
-          const int64_t off = r < cur.it.rows ? (int64_t)(cur.s.q0 + token) * a.qs + (int64_t)(cur.h * a.p.group + rr - token * a.p.group) * D : -1;
+          const int64_t off = r < cur.it.rows ? (int64_t)(cur.s.q0 + token) * a.qs + (int64_t)(cur.h * a.p.group + rr - token * a.p.group) * c.d : -1;
 #pragma unroll 4
           for (int y = 0; y < 32; y += R::RPI) {
             const int64_t o = __shfl_sync(0xffffffffu, off, y + my_row);
-            cp_async16_zfill(sq + (x >> 7) * K::TILE + R::off((x & 127) + y + my_row, ch), static_cast<const T*>(a.q) + (o < 0 ? 0 : o) + ch * 8,
-                             o >= 0);
+            const bool there = o >= 0 && ch * 8 < c.d;
+            cp_async16_zfill(sq + (x >> 7) * K::TILE + R::off((x & 127) + y + my_row, ch), static_cast<const T*>(a.q) + (there ? o + ch * 8 : 0),
+                             there);
           }
         }
         cp_async_commit();
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
           const int rr = it.r0 + row, token = plan_token(a.p, rr);
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           T* out = static_cast<T*>(a.out) + (int64_t)(it.s.q0 + token) * a.os +
-                   (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D;
+                   (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d;
           bool bad = false;
 #pragma unroll 1
           for (int x = 0; x < D; x += 32) {
@@ -514,6 +519,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
             if (row < it.rows) {
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
+                if (x + e >= c.d) break;
                 uint32_t p[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {

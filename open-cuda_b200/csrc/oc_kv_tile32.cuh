@@ -1,5 +1,5 @@
 // oc_kv_tile32.cuh -- attention over the paged cache for chunks of new tokens
-// in f32, head_dim 64 and 128, on the tcgen05 tensor cores.
+// in f32 on the tcgen05 tensor cores (D: head_dim, or 64 or 128 above it).
 //
 // The arithmetic is flash_tc_kernel's (oc_flash_tc.cuh): every operand as two
 // f16 terms of a power-of-two scaling (Q and K per row, V per tile, P by
@@ -13,10 +13,10 @@
 // Bound: not the tensor pipe but the chain of a tile, S -> softmax (two passes
 // over tensor memory) -> P V -> next S, about 8000 cycles at d = 64, and the
 // conversion of K and V beside it.  Measured: 8 prompts of 300 to 777 tokens
-// over contexts of 800 to 1000, 12 heads of 64: 143 us a call (55 TFLOP/s of
+// over contexts of 800 to 1000, 12 heads of 64: 125 us a call (63 TFLOP/s of
 // visible products; the CUDA cores took 1220).  S in two buffers with K
-// converted a tile ahead measured slower (167 us: the softmax warps, which
-// share their schedulers with the converters, spill).
+// converted a tile ahead measured slower (167 us : 143 then: the softmax
+// warps, which share their schedulers with the converters, spill).
 //
 // One CTA an SM, 448 threads:
 //   warp 0       TMEM allocator + MMA issuer (lane 0)
@@ -56,7 +56,7 @@ struct KvTile32Shared {
 // see both do not mind; one that sees the smaller alone does, so this is
 // asked of tiles that some row sees in part.
 template <int D, bool TILE>
-__device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, int64_t off, bool vec, uint8_t* thi,
+__device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, int64_t off, int d, bool vec, uint8_t* thi,
                                                 uint8_t* tlo, float* inv, float sign, int w, int lane, float* part,
                                                 uint64_t* vmax, uint32_t ph, volatile int* abort_flag,
                                                 uint32_t* rough = nullptr, uint32_t id = 0) {
@@ -67,12 +67,13 @@ __device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, 
   for (int s = 0; s < NS; ++s) {
     const int64_t o = __shfl_sync(0xffffffffu, off, s * RPS + ro);
     x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (o >= 0) {
+    if (o >= 0 && 4 * q4 < d) {
       const float* p = base + o + 4 * q4;
+      const int left = d - 4 * q4;  // zeros behind head_dim
       if (vec)
         x[s] = *reinterpret_cast<const float4*>(p);
       else
-        x[s] = make_float4(p[0], p[1], p[2], p[3]);
+        x[s] = make_float4(p[0], left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
     }
   }
   float cr[NS];
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
           auto terms = [&](const uint8_t* q, const uint8_t* k, uint32_t first) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
+              if (kk * 16 >= c.d) break;
               const uint32_t off = (uint32_t)(kk >> 2) * K::PANEL + (uint32_t)(kk & 3) * 32;
               mma_f16(tmem + K::S_COL, desc_kmajor_sw128(smem_u32(q) + off), desc_kmajor_sw128(smem_u32(k) + off), idesc_s,
                       first && kk == 0 ? 0u : 1u);
@@ -264,8 +266,8 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
       ok = warp_wait(&sh.q_empty, (items & 1) ^ 1, abort_flag);
       if (!ok) break;
       const int rr = it.r0 + mine, token = plan_token(a.p, rr);
-      const int64_t qoff = mine < it.rows ? (int64_t)(it.s.q0 + token) * a.qs + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D : -1;
-      kv_convert_tile<D, false>(static_cast<const float*>(a.q), qoff, a.qvec, q_hi, q_lo, sh.icq[items & 1], 1.0f, w, lane, nullptr, nullptr, 0,
+      const int64_t qoff = mine < it.rows ? (int64_t)(it.s.q0 + token) * a.qs + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d : -1;
+      kv_convert_tile<D, false>(static_cast<const float*>(a.q), qoff, c.d, a.qvec, q_hi, q_lo, sh.icq[items & 1], 1.0f, w, lane, nullptr, nullptr, 0,
                                 abort_flag);
       fence_proxy_async_smem();
       __syncwarp();
@@ -281,14 +283,14 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         if (t + 1 < it.t1) next = kv_row_off(a, it.s.s, it.h, (it.tile0 + t + 1) * K::BK + mine, it.lo, it.hi);
         ok = warp_wait(&sh.k_empty, ph ^ 1u, abort_flag);
         if (!ok) break;
-        kv_convert_tile<D, false>(kb, off, a.vec, k_hi, k_lo, sh.ick[ph], ksign, w, lane, nullptr, nullptr, 0, abort_flag);
+        kv_convert_tile<D, false>(kb, off, c.d, a.vec, k_hi, k_lo, sh.ick[ph], ksign, w, lane, nullptr, nullptr, 0, abort_flag);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full);
         const int first = max((it.tile0 + t) * K::BK, it.lo), last = min((it.tile0 + t + 1) * K::BK, it.hi);
         const bool masked = first < all_lo || last > all_hi;  // (zeros stand in place of keys that no row sees)
         ok = warp_wait(&sh.v_empty, ph ^ 1u, abort_flag) &&
-             kv_convert_tile<D, true>(vb, off, a.vec, v_hi, v_lo, &sh.icv[ph], 1.0f, w, lane, sh.vpart[ph], &sh.vmax, ph, abort_flag,
+             kv_convert_tile<D, true>(vb, off, c.d, a.vec, v_hi, v_lo, &sh.icv[ph], 1.0f, w, lane, sh.vpart[ph], &sh.vmax, ph, abort_flag,
                                       masked ? &sh.rough[items & 1] : nullptr, items + 1);
         if (!ok) break;
         fence_proxy_async_smem();
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
       const bool whole = t0 == 0 && t1 == it.units, rough = *reinterpret_cast<volatile uint32_t*>(&sh.rough[items & 1]) == items + 1;
       const int rr = it.r0 + row, token = plan_token(a.p, rr);
       const float inv = l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
-      float* dst = whole ? static_cast<float*>(a.out) + (int64_t)(it.s.q0 + token) * a.os + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * D
+      float* dst = whole ? static_cast<float*>(a.out) + (int64_t)(it.s.q0 + token) * a.os + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d
                          : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D) + plan_slot_o(K::ROWS) + (size_t)row * D;
       const bool vec = !whole || a.ovec16;
       if (!whole && row < it.rows) {
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         if (row < it.rows) {
 #pragma unroll
           for (int f = 0; f < 32; f += 4) {
+            if (whole && cb * 32 + f >= c.d) break;
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -420,7 +423,8 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
               *reinterpret_cast<float4*>(dst + cb * 32 + f) = make_float4(y[0], y[1], y[2], y[3]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) dst[cb * 32 + f + e] = y[e];
+              for (int e = 0; e < 4; ++e)
+                if (cb * 32 + f + e < c.d) dst[cb * 32 + f + e] = y[e];
             }
           }
         }

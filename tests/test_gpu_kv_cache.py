@@ -224,6 +224,16 @@ def test_unaligned_queries_and_pools(dtype):
     close(attend(moved, q, [0, 1], [1, 3]), want, tol)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq, hk, d", [(4, 2, 40), (6, 2, 72), (3, 3, 80), (10, 2, 96), (2, 1, 120), (4, 2, 24), (3, 1, 33)])
+@pytest.mark.parametrize("page", [4, 16, 128])
+def test_padded_heads_in_one_call(dtype, hq, hk, d, page):
+    """Head sizes between the tiles' widths: single tokens and chunks side by
+    side, both with items that cuts go through, and pages that end in a tile."""
+    check(dtype, hq, hk, d, page, [3000, 700, 2501, 129], [1, 300, 1, 129], seed=d, layers=2, layer=1)
+    check(dtype, hq, hk, d, page, [1500, 900], [5, 260], causal=False, window=333, seed=d + 1)
+
+
 @pytest.mark.parametrize("dtype, big", [(F32, 3e38), (F16, 65504.0), (BF16, torch.finfo(BF16).max)])
 @pytest.mark.parametrize("hq, hk, d", [(8, 2, 64), (4, 2, 128), (4, 2, 80), (2, 2, 256), (3, 1, 17)])
 @pytest.mark.parametrize("lens, new", [([9, 40], [1, 1]), ([3000], [1]), ([300, 1500], [20, 100]), ([2100], [260])])
