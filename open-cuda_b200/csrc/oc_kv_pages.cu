@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (threadIdx.x == 0) err = 0;
   for (int i = threadIdx.x; i < (c.max_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
   __syncthreads();
-  int need = 0;  // pages taken by the entries before this round's (saturating: more than the pool is refused)
+  int need = 0;  // pages taken by the entries before this pass's (saturating: more than the pool is refused)
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + threadIdx.x;
     int want = 0;
