@@ -200,7 +200,7 @@ struct KvLaunch {
   void (*kern)(KvAttn) = nullptr;
   void (*tile)(KvAttn, CUtensorMap, CUtensorMap, CUtensorMap, int, int) = nullptr;  // or this one
   const void* fn() const { return kern ? reinterpret_cast<const void*>(kern) : reinterpret_cast<const void*>(tile); }
-  int br = 0, bk = 0, dp = 0, threads = 0, min_units = 1;
+  int br = 0, bk = 0, dp = 0, threads = 0;
   int rows_min = 0, rows_max = INT_MAX;
   size_t smem = 0;
   int ctas = 0;
@@ -209,20 +209,23 @@ struct KvLaunch {
 };
 
 template <typename K>
-static KvLaunch shape_of(void (*kern)(KvAttn), int min_units) {
+static KvLaunch shape_of(void (*kern)(KvAttn)) {
   KvLaunch l;
   l.kern = kern;
-  l.br = K::ROWS, l.bk = K::BK, l.dp = K::DP, l.threads = K::THREADS, l.min_units = min_units, l.smem = K::SMEM;
+  l.br = K::ROWS, l.bk = K::BK, l.dp = K::DP, l.threads = K::THREADS, l.smem = K::SMEM;
   return l;
 }
 
 // On the CUDA cores; `rows`: the most that a sequence's kv head can have.
+// The rows of an item are the registers' and the multiply-adds' cost, used or
+// not: one token over 20000 keys, 32 f32 heads of 128 over 8, takes 75 us in
+// items of 4 rows (2.2 TB/s; multiply-adds bound it) and 153 in items of 8.
 template <typename T>
 static KvLaunch scalar_launch(int d, int rows) {
-  auto go = [](auto k) { return shape_of<decltype(k)>(kv_rows_kernel<decltype(k)>, 4); };
+  auto go = [](auto k) { return shape_of<decltype(k)>(kv_rows_kernel<decltype(k)>); };
   if constexpr (sizeof(T) == 4) {
-    if (d <= 64) return rows <= 1 ? go(KvRows<T, 64, 1>()) : go(KvRows<T, 64, 8>());
-    if (d <= 128) return rows <= 1 ? go(KvRows<T, 128, 1>()) : go(KvRows<T, 128, 8>());
+    if (d <= 64) return rows <= 1 ? go(KvRows<T, 64, 1>()) : rows <= 4 ? go(KvRows<T, 64, 4>()) : go(KvRows<T, 64, 8>());
+    if (d <= 128) return rows <= 1 ? go(KvRows<T, 128, 1>()) : rows <= 4 ? go(KvRows<T, 128, 4>()) : go(KvRows<T, 128, 8>());
     return go(KvRows<T, 256, 4>());
   } else {
     if (d <= 64) return go(KvRows<T, 64, 4>());
@@ -234,7 +237,7 @@ static KvLaunch scalar_launch(int d, int rows) {
 // On warp-level matrix instructions.
 template <typename T>
 static KvLaunch mma_launch(int d, int rows) {
-  auto go = [](auto k) { return shape_of<decltype(k)>(kv_mma_kernel<decltype(k)>, 1); };
+  auto go = [](auto k) { return shape_of<decltype(k)>(kv_mma_kernel<decltype(k)>); };
   if (d <= 64) return rows <= 16 ? go(KvMma<T, 64, 1>()) : go(KvMma<T, 64, 2>());
   if (d <= 96) return rows <= 16 ? go(KvMma<T, 96, 1>()) : go(KvMma<T, 96, 2>());
   if (d <= 128) return rows <= 16 ? go(KvMma<T, 128, 1>()) : go(KvMma<T, 128, 2>());
@@ -281,11 +284,11 @@ static int pick(const KvView& c, int tokens, int n, int q_heads, bool one_each, 
       out[count++].rows_max = few;
     }
     if constexpr (sizeof(T) == 4) {
-      auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>, 2); };
+      auto go = [](auto k) { return shape_of<decltype(k)>(kv_tile32_kernel<decltype(k)>); };
       out[count] = c.d <= 64 ? go(KvTile32<64>()) : go(KvTile32<128>());
     } else {
       auto go = [](auto k) {
-        KvLaunch l = shape_of<decltype(k)>(nullptr, 2);
+        KvLaunch l = shape_of<decltype(k)>(nullptr);
         l.tile = kv_tile_kernel<decltype(k)>;
         return l;
       };
@@ -324,7 +327,7 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
   int dp = 0, rows = 0;
   for (int i = 0; i < count; ++i) {
     a.p.br = l[i].br, a.p.bk_shift = __builtin_ctz(l[i].bk), a.p.rows_min = l[i].rows_min, a.p.rows_max = l[i].rows_max;
-    a.p.ctas = l[i].ctas, a.p.min_units = l[i].min_units;
+    a.p.ctas = l[i].ctas;
     a.beside = i > 0;
     if (!smem_attr_once(l[i].fn(), l[i].smem)) return fail(OC_ERR_LAUNCH_FAILED, "kv_attention: shared memory attribute refused");
     const dim3 grid(l[i].ctas), block(l[i].threads);
