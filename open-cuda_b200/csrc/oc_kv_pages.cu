@@ -64,6 +64,19 @@ __device__ int find_free(const int* refs, int pages, int need, int* list, int* w
   return min(found, need);
 }
 
+// The pages that an accepted list needs, into list; *err (shared) becomes
+// kKvNoPages when there are too few.  All threads, behind a barrier that
+// follows the last write to *err.  Every thread reads *err before any writes
+// it again: what follows has barriers, so all have to go the same way.
+__device__ __forceinline__ void plan_pages(const KvView& c, int need, int* list, int* warp_sums, int* err) {
+  const bool go = *err == 0 && need > 0;
+  __syncthreads();
+  if (!go) return;
+  const int found = need > c.pages ? 0 : find_free(c.refs, c.pages, need, list, warp_sums);
+  if (found < need && threadIdx.x == 0) *err = kKvNoPages;
+  __syncthreads();
+}
+
 __device__ __forceinline__ int pages_of(int tokens, int ps_shift) {
   return (int)(((int64_t)tokens + (1 << ps_shift) - 1) >> ps_shift);
 }
@@ -107,11 +120,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     need = (int)min((int64_t)need + total, (int64_t)c.pages + 1);
   }
   __syncthreads();
-  if (err == 0 && need > 0) {
-    const int found = need > c.pages ? 0 : find_free(c.refs, c.pages, need, sc.list, sums);
-    if (found < need && threadIdx.x == 0) err = kKvNoPages;
-    __syncthreads();
-  }
+  plan_pages(c, need, sc.list, sums, &err);
   if (err) {
     if (threadIdx.x == 0) atomicOr(c.status, err);
     return;
@@ -169,11 +178,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     need += total;
   }
   __syncthreads();
-  if (err == 0 && need > 0) {
-    const int found = need > c.pages ? 0 : find_free(c.refs, c.pages, need, sc.list, sums);
-    if (found < need && threadIdx.x == 0) err = kKvNoPages;
-    __syncthreads();
-  }
+  plan_pages(c, need, sc.list, sums, &err);
   if (threadIdx.x == 0) {
     sc.head[0] = err ? -1 : need;
     if (err) atomicOr(c.status, err);
@@ -356,7 +361,9 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (s < 0 || s >= c.pages || d < 0 || d >= c.pages || mark(bits, d)) err = kKvBadPage;
   }
   __syncthreads();
-  if (err == 0)
+  const bool in_pool = err == 0;
+  __syncthreads();  // all have read it before it is written again
+  if (in_pool)
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
       const int s = src[i];
       if (s != dst[i] && ((bits[s >> 5] >> (s & 31)) & 1u)) err = kKvBadPage;

@@ -738,6 +738,26 @@ def test_refused_calls_change_nothing():
     c.check()
 
 
+def test_more_pages_than_the_pool_has():
+    """Lists that need more pages than there are at all: refused before the
+    free ones are looked for, by every warp alike."""
+    for _ in range(20):
+        c, b = fresh(4, 16, 40, 64)
+        c.extend(ints([0]), ints([5]))
+        b.extend([0], [5])
+        before = state(c)
+        for call in (lambda: c.extend(ints([1]), ints([16 * 5])), lambda: c.extend(ints(range(1, 40)), ints([1] * 39)),
+                     lambda: c.extend(ints([1, 2]), ints([16 * 60, 16 * 60])), lambda: c.fork(ints([0] * 30), ints(range(1, 31)))):
+            call()
+            assert all(torch.equal(x, y) for x, y in zip(state(c), before))
+            with pytest.raises(ValueError, match="too few"):
+                c.check()
+        c.extend(ints([1]), ints([16 * 3]))
+        b.extend([1], [16 * 3])
+        b.same(c)
+        c.check()
+
+
 def test_copy_pages():
     c, _ = fresh(50, 8, 4, 4, layers=3)
     k, v = c.k.clone(), c.v.clone()
