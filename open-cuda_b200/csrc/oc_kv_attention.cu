@@ -31,7 +31,8 @@ struct KvParts {
 template <typename T, int R, int DP>
 __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts) {
   constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
-  __shared__ float part[R == 1 ? WARPS : 1][DP], ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
+  __shared__ alignas(16) float part[R == 1 ? WARPS : 1][DP];  // written four features at a time
+  __shared__ float ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
   __shared__ unsigned short list[2][kMostCtas];
   __shared__ int wcount[2][WARPS];
   const KvView& c = a.c;

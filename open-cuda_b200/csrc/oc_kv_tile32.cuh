@@ -24,6 +24,8 @@
 //   warps 9..12  softmax and output: thread = query row = TMEM lane
 //   warp 13      walks the CTA's run and hands its pieces to the others
 #pragma once
+#include <cstddef>
+
 #include "oc_kv_tile.cuh"
 
 namespace oc {
@@ -40,14 +42,15 @@ struct KvTile32Shared {
   uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_full, o_empty, vmax;
   uint64_t job_full[kJobs], job_empty[kJobs];
   KvJob ring[kJobs];
-  float icq[2][128];       // 1 / c_q per query row, by the piece's parity
-  float ick[2][128];       // 1 / c_k per key row, with the sign of the scale, by the tile's parity
+  float icq[2][128];              // 1 / c_q per query row, by the piece's parity
+  alignas(16) float ick[2][128];  // 1 / c_k per key row, with the sign of the scale, by the tile's parity (read four at a time)
   float icv[2];            // 1 / c_v of the V tile
   float vpart[2][kFaConv]; // converter warps' max |v|
   uint32_t rough[2];       // by the piece's parity: its number + 1 when V's rows are too uneven for its masks
   uint32_t tmem;
   int abort_word;
 };
+static_assert(offsetof(KvTile32Shared, ick) % 16 == 0 && alignof(KvTile32Shared) % 16 == 0, "ick is read as float4");
 
 // The converter warp's 16 rows of a 128-row tile, from the offsets that its
 // lanes 0..15 hold (-1: a row of zeros): fa_convert_tile with rows anywhere.
