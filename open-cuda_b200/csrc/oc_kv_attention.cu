@@ -13,11 +13,64 @@ constexpr int kMostCtas = 2048;  // of an attention kernel's grid
 struct KvPart {
   float* ws;
   int ctas, br, groups, dp;  // groups: of R rows, that an item can have; dp: floats of a row
+  KvPlan p;
 };
 struct KvParts {
   KvPart of[2];
   int count;
 };
+
+// Rows whose result is not finite, from the definition (oc_kv_rows.cuh): those
+// of this merge CTA's tasks, and its share of those that the attention kernels
+// left in their whole items.  All threads of the CTA.
+template <typename T, int R, int DP>
+__device__ __noinline__ void kv_merge_exact(const KvAttn& a, const KvParts& parts, unsigned short* list0, const unsigned short* list1,
+                                            int tasks0, int tasks, float* meet) {
+  __shared__ KvPlanShared plan;
+  auto row = [&](KvSeq s, int h, int r) {
+    if (__syncthreads_or(kv_row_lost<T>(a, s, h, r, threadIdx.x, blockDim.x))) kv_row_exact<T, DP>(a, s, h, r, meet);
+  };
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const bool second = task >= tasks0;
+    const KvPart& pt = parts.of[second];
+    const int number = second ? task - tasks0 : task;
+    const KvCut cut = reinterpret_cast<const KvCut*>(pt.ws)[(second ? list1 : list0)[number / pt.groups]];
+    const KvSeq s = kv_seq(a.c, a.bt, cut.b);
+    const int r0 = number % pt.groups * R, r1 = min(cut.rows, r0 + R);
+    for (int r = r0; r < r1; ++r) row(s, cut.h, cut.r0 + r);
+  }
+  for (int k = 0; k < parts.count; ++k) {
+    const KvPart& pt = parts.of[k];
+    // the attention CTAs that lost some, in order
+    int found = 0;
+    for (int c0 = 0; c0 < pt.ctas; c0 += blockDim.x) {
+      const int cta = c0 + threadIdx.x;
+      const int lost = cta < pt.ctas && reinterpret_cast<const KvCut*>(pt.ws)[cta].lost;
+      int64_t sum;
+      const int at = found + (int)block_exclusive<int64_t>(lost, plan.sums, &sum);
+      if (lost) list0[at] = (unsigned short)cta;
+      found += (int)sum;
+    }
+    __syncthreads();
+    // each one's rows are shared by as many CTAs as there are for it
+    const int shares = max(1, (int)gridDim.x / max(1, found));
+    for (int job = blockIdx.x; job < found * shares; job += gridDim.x) {
+      const int cta = list0[job % found], share = job / found;
+      KvCursor cur;
+      int64_t chunk;
+      const int64_t total = plan_locate(pt.p, a.c, a.bt, cta, &plan, &chunk, cur);
+      for (int64_t left = min(chunk, total - chunk * cta); left > 0;) {
+        const int t1 = (int)min((int64_t)cur.it.units, cur.at + left);
+        if (cur.at == 0 && t1 == cur.it.units)
+          for (int r = share; r < cur.it.rows; r += shares) row(cur.s, cur.h, cur.it.r0 + r);
+        left -= t1 - cur.at;
+        if (left > 0) plan_next(pt.p, a.c, a.bt, cur);
+      }
+      __syncthreads();  // (plan_locate's shared memory)
+    }
+    __syncthreads();
+  }
+}
 
 // Joins the pieces of the items that cuts went through.  R rows of an item at
 // a time: one, its pieces shared by the 8 warps, for decode steps, where an
@@ -29,10 +82,11 @@ struct KvParts {
 // would mostly be launched to find nothing (2065 CTAs, 8 us, at 296 x 7).
 // DP: features of a row, 128 or 256.
 template <typename T, int R, int DP>
-__global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts) {
+__global__ void __launch_bounds__(256, R == 1 ? 2 : 4) kv_merge_kernel(const __grid_constant__ KvAttn a, const __grid_constant__ KvParts parts) {
   constexpr int WARPS = 8, SPLIT = WARPS / R, NV = DP / 128;  // warps that share a row
-  __shared__ alignas(16) float part[R == 1 ? WARPS : 1][DP];  // written four features at a time
-  __shared__ float ms[R == 1 ? WARPS : 1], ls[R == 1 ? WARPS : 1];
+  __shared__ alignas(16) float meet[kv_exact_floats(32 * WARPS, DP)];  // R == 1: rows of outputs, written four features at a time, maxima and sums
+  float(*part)[DP] = reinterpret_cast<float(*)[DP]>(meet);
+  float *ms = meet + WARPS * DP, *ls = ms + WARPS;
   __shared__ unsigned short list[2][kMostCtas];
   __shared__ int wcount[2][WARPS];
   const KvView& c = a.c;
@@ -42,6 +96,7 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
   // order of the list does not matter
   constexpr int ROUNDS = kMostCtas / 256;
   uint32_t mine[2] = {0, 0};
+  int lost = 0;  // a result that is not finite
   int before[2], found[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -50,7 +105,10 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) {
         const int cta = i * 256 + threadIdx.x;
-        if (cta < parts.of[k].ctas && cuts[cta].pieces > 0) mine[k] |= 1u << i;
+        if (cta < parts.of[k].ctas) {
+          if (cuts[cta].pieces > 0) mine[k] |= 1u << i;
+          lost |= cuts[cta].lost;
+        }
       }
     }
     before[k] = __popc(mine[k]);
@@ -131,7 +189,6 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
     }
     const int rr = cut.r0 + r, token = plan_token(a.p, rr);
     T* out = static_cast<T*>(a.out) + (int64_t)(cut.q0 + token) * a.os + (int64_t)(cut.h * a.p.group + rr - token * a.p.group) * d;
-    bool bad = false;
     if constexpr (R == 1) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) *reinterpret_cast<float4*>(&part[warp][128 * k + 4 * lane]) = acc[k];
@@ -151,9 +208,9 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
         }
         o = sum == 0.0f ? 0.0f : o / sum;
         out[threadIdx.x] = kv_from<T>(o);
-        bad = kv_lost<T>(o);
+        lost |= kv_lost<T>(o);
       }
-      bad = __syncthreads_or(bad) && warp == 0;
+      __syncthreads();
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -164,17 +221,13 @@ __global__ void __launch_bounds__(256) kv_merge_kernel(const __grid_constant__ K
           if (x < d) {
             const float o = l == 0.0f ? 0.0f : f[e] / l;
             out[x] = kv_from<T>(o);
-            bad |= kv_lost<T>(o);
+            lost |= kv_lost<T>(o);
           }
         }
       }
-      bad = __any_sync(0xffffffffu, bad);
-      __syncwarp();  // the row is written again, by other lanes
     }
-    // (oc_kv_rows.cuh) a row that was lost is computed from the definition
-    if (bad) kv_row_exact<T>(a, kv_seq(c, a.bt, cut.b), cut.h, rr);
-    if constexpr (R == 1) __syncthreads();
   }
+  if (__syncthreads_or(lost)) kv_merge_exact<T, R, DP>(a, parts, list[0], list[1], tasks0, tasks, meet);
 }
 
 // CTAs of a kernel that fit the GPU at once, remembered per device and kernel.
@@ -353,7 +406,7 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
           return rc;
       OC_CHECK_CUDA(launch_pdl_ex(l[i].tile, grid, block, l[i].smem, s, a, m[0], m[1], m[2], box, qbox));
     }
-    parts.of[i] = KvPart{a.ws, l[i].ctas, l[i].br, 0, l[i].dp};
+    parts.of[i] = KvPart{a.ws, l[i].ctas, l[i].br, 0, l[i].dp, a.p};
     a.ws += part_floats(l[i]);
     dp = std::max(dp, l[i].dp);
     rows = std::max(rows, l[i].merge_rows);
@@ -366,8 +419,7 @@ static int run(KvAttn a, int q_heads, bool one_each, void* ws, size_t ws_bytes, 
     parts.of[i].groups = few ? l[i].merge_rows : (l[i].merge_rows + 7) / 8;
     tasks += (int64_t)(l[i].ctas - 1) * parts.of[i].groups;
   }
-  if (tasks == 0) return OC_OK;  // one CTA: nothing is cut
-  const int grid = (int)std::min<int64_t>(tasks, (few ? 4 : 8) * (int64_t)std::max(1, sm_count()));
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(tasks, (few ? 4 : 8) * (int64_t)std::max(1, sm_count())));
   auto go = [&](auto kern) {
     OC_CHECK_CUDA(launch_pdl_ex(kern, dim3(grid), dim3(256), 0, s, a, parts));
     return OC_OK;

@@ -20,7 +20,7 @@
 //               the result then differs from f32 arithmetic by less than its
 //               own last rounding
 // A weight of a key that a row does not see is 0, but 0 times an infinity or
-// NaN is NaN: a row whose result is not finite is computed again, key by key
+// NaN is NaN: a row whose result is not finite is computed again
 // (kv_row_exact), so that what it does not see has no part in it.
 #pragma once
 #include "oc_kv_rows.cuh"
@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
   const uint32_t v_off = (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * L::RB + (lane >> 4) * 16);
   const uint32_t q_off = (uint32_t)((lane & 15) * L::RB + (lane >> 4) * 16);
 
+  bool lost = false;  // a result of this thread's is not finite
   while (left > 0) {
     const KvItem& it = cur.it;
     const int t0 = cur.at, t1 = (int)min((int64_t)it.units, t0 + left);
@@ -298,7 +299,6 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
       }
     __syncthreads();
     float* slot = whole ? nullptr : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, DP);
-    uint32_t bad = 0;  // rows with a result that is not finite
     for (int x = threadIdx.x; x < it.rows * (DP / 2); x += K::THREADS) {
       const int r = x / (DP / 2), e = x % (DP / 2) * 2;
       float mm = pm[0][r];
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
         if (e < d) {
           const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
           os.x *= inv, os.y *= inv;
-          if (kv_lost<T>(os.x) || kv_lost<T>(os.y)) bad |= 1u << r;
+          lost |= kv_lost<T>(os.x) || kv_lost<T>(os.y);
           T* out = static_cast<T*>(a.out) + (int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.os + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e;
           if (a.ovec) {
             *reinterpret_cast<uint32_t*>(out) = kv_pack2<T>(os.x, os.y);
@@ -334,21 +334,12 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
         *reinterpret_cast<float2*>(slot + plan_slot_o(ROWS) + (size_t)r * DP + e) = os;
       }
     }
-    if (__syncthreads_or(bad != 0)) {
-      uint32_t* rows = reinterpret_cast<uint32_t*>(pm);
-      if (threadIdx.x == 0) *rows = 0;
-      __syncthreads();
-      if (bad) atomicOr(rows, bad);
-      __syncthreads();
-      const uint32_t todo = *rows;
-      for (int r = warp; r < it.rows; r += K::WARPS)
-        if ((todo >> r) & 1u) kv_row_exact<T>(a, cur.s, cur.h, it.r0 + r);
-      __syncthreads();
-    }
+    __syncthreads();
     if (t0 == 0 && !whole && threadIdx.x == 0) plan_cut(a, cur, it.units - t1, chunk);
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }
+  plan_lost(a, lost);
 }
 
 }  // namespace oc

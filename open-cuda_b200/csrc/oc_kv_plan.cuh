@@ -229,10 +229,11 @@ __device__ __forceinline__ bool plan_next(const KvPlan& p, const KvView& c, cons
   return true;
 }
 
-// What the cut behind a CTA's run goes through, for the merge kernel.
+// What the cut behind a CTA's run goes through, and whether a result of the
+// run's whole items is not finite, for the merge kernel.
 struct KvCut {
   int pieces;  // 0: nothing
-  int b, h, r0, rows, q0, unused0, unused1;
+  int b, h, r0, rows, q0, lost, unused;
 };
 
 // Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp]
@@ -266,12 +267,19 @@ __device__ __forceinline__ float* plan_slot(const KvAttn& a, int cta, int slot, 
 
 // One thread of a CTA: what its run leaves to the CTAs behind it.
 __device__ __forceinline__ void plan_no_cut(const KvAttn& a) {
-  reinterpret_cast<KvCut*>(a.ws)[blockIdx.x].pieces = 0;
+  KvCut& cut = reinterpret_cast<KvCut*>(a.ws)[blockIdx.x];
+  cut.pieces = cut.lost = 0;
 }
 // The last item of its run began there and goes on: rest = its units behind the run.
 __device__ __forceinline__ void plan_cut(const KvAttn& a, const KvCursor& cur, int rest, int64_t chunk) {
   reinterpret_cast<KvCut*>(a.ws)[blockIdx.x] =
       KvCut{2 + (int)((rest - 1) / chunk), cur.b, cur.h, cur.it.r0, cur.it.rows, cur.s.q0, 0, 0};
+}
+// All threads, the last to write there: `lost` of any of them.  Such rows are
+// computed again by the merge kernel: it has no waits that would run out, and
+// the whole GPU for them.
+__device__ __forceinline__ void plan_lost(const KvAttn& a, bool lost) {
+  if (__syncthreads_or(lost) && threadIdx.x == 0) reinterpret_cast<KvCut*>(a.ws)[blockIdx.x].lost = 1;
 }
 
 }  // namespace oc

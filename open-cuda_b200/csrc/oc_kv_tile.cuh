@@ -43,8 +43,9 @@
 // P is rounded once to the operands' type (bf16: 2^-9 at most, as much as the
 // result's own rounding); sums and maxima are f32, the sum of P is taken
 // before the rounding.  Rows that are not finite, or would not be once rounded,
-// are computed again from the definition (kv_row_exact): a zero weight does
-// not hide a NaN or an infinity of a key that the row does not see.
+// are computed again from the definition (kv_row_exact), by the merge kernel:
+// here the other warps' waits would run out.  A zero weight does not hide a
+// NaN or an infinity of a key that the row does not see.
 #pragma once
 #include "oc_flash_tc.cuh"
 #include "oc_kv_mma.cuh"
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   KvJobs<KvTileBars> jobs{ring, &bar};
+  bool lost = false;  // a result of this thread's is not finite
 
   if (warp == 0) {
     if (lane == 0) {
@@ -510,7 +512,6 @@ __global__ void __launch_bounds__(K::THREADS, 1)
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           T* out = static_cast<T*>(a.out) + (int64_t)(it.s.q0 + token) * a.os +
                    (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d;
-          bool bad = false;
 #pragma unroll 1
           for (int x = 0; x < D; x += 32) {
             uint32_t o[32];
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const float y0 = __uint_as_float(o[e + 2 * k]) * inv, y1 = __uint_as_float(o[e + 2 * k + 1]) * inv;
-                  bad |= kv_lost<T>(y0) || kv_lost<T>(y1);
+                  lost |= kv_lost<T>(y0) || kv_lost<T>(y1);
                   p[k] = kv_pack2<T>(y0, y1);
                 }
                 if (a.ovec16) {
@@ -536,9 +537,6 @@ __global__ void __launch_bounds__(K::THREADS, 1)
               }
             }
           }
-          __syncwarp();
-          for (uint32_t todo = __ballot_sync(0xffffffffu, bad); todo; todo &= todo - 1)
-            kv_row_exact<T>(a, it.s, it.h, it.r0 + sub * 128 + quad * 32 + __ffs(todo) - 1);
         } else {
           float* slot = plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D);
           if (row < it.rows) slot[row] = m, slot[K::ROWS + row] = l;
@@ -563,7 +561,7 @@ __global__ void __launch_bounds__(K::THREADS, 1)
     if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutEpilogue);
   }
   tc_fence_before();
-  __syncthreads();
+  plan_lost(a, lost);
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, K::TMEM_COLS);

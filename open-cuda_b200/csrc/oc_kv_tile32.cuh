@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   KvJobs<KvTile32Shared> jobs{sh.ring, &sh};
+  bool lost = false;  // a result of this thread's is not finite
 
   if (warp == 0) {
     if (lane == 0) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
       if (!ok) break;
       const bool whole = t0 == 0 && t1 == it.units, rough = *reinterpret_cast<volatile uint32_t*>(&sh.rough[items & 1]) == items + 1;
       const int rr = it.r0 + row, token = plan_token(a.p, rr);
-      const float inv = l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
+      const float inv = rough ? NAN : l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
       float* dst = whole ? static_cast<float*>(a.out) + (int64_t)(it.s.q0 + token) * a.os + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d
                          : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D) + plan_slot_o(K::ROWS) + (size_t)row * D;
       const bool vec = !whole || a.ovec16;
@@ -402,7 +403,6 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         float* slot = plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D);
         slot[row] = m_i, slot[K::ROWS + row] = rough ? NAN : l_i;  // the merge computes such rows again
       }
-      bool bad = whole && rough && row < it.rows;
 #pragma unroll 1
       for (int cb = 0; cb < D / 32; ++cb) {
         uint32_t o[32];
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
               if (whole) {
                 // the quotient with one rounding more than the division's
                 y[e] = __fmul_rn(y[e], inv);
-                bad |= !isfinite(y[e]);
+                lost |= !isfinite(y[e]);
               }
             }
             if (vec) {
@@ -432,10 +432,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
           }
         }
       }
-      const uint32_t rows_bad = __ballot_sync(0xffffffffu, bad);
       __syncwarp();
-      for (uint32_t todo = rows_bad; todo; todo &= todo - 1)
-        kv_row_exact<float>(a, it.s, it.h, it.r0 + quad * 32 + __ffs(todo) - 1);
       tc_fence_before();  // the running output's columns belong to these warps alone
       ++items;
       jobs.template drop<true>();
@@ -456,7 +453,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
     if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
   }
   tc_fence_before();
-  __syncthreads();
+  plan_lost(a, lost);
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, K::TMEM_COLS);

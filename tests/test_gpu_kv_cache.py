@@ -334,6 +334,37 @@ def test_nonfinite_values_that_are_seen(dtype):
         assert torch.isfinite(o).all()
 
 
+@pytest.mark.parametrize("dtype, hq, hk", [(F32, 12, 12), (F16, 28, 4), (BF16, 28, 4)])
+def test_an_infinite_value_in_view_of_a_long_chunk(dtype, hq, hk):
+    """Every row of 2048 new tokens over 60000 keys sees one infinite value and
+    is computed again; the rows of the sequences beside it, and the other
+    features, are what they are without it.  Two results of one row differ by
+    what each may be off: A (the weighted mean of |v|) is below 1 over so many
+    standard normal values, and expected() is asked for rows all over."""
+    n, new, d = 60000, 2048, 64
+    c, ks, vs = filled(dtype, hk, d, 64, [400, n, 300])
+    parts = [300, new, 5]
+    q = torch.randn(sum(parts), hq, d, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(dtype)
+    without = attend(c, q, [0, 1, 2], parts)
+    page = int(c.page_table[1, 1000 // 64])
+    c.v[0, page, :, 1000 % 64, 5] = math.inf
+    o = attend(c, q, [0, 1, 2], parts, out=torch.full_like(q, 7.0))
+    c.check()
+    again = o[300:300 + new]
+    assert (again[:, :, 5] == math.inf).all()
+    rest = [f for f in range(d) if f != 5]
+    for s, at in ((0, 0), (2, 300 + new)):
+        rows = slice(at, at + parts[s])
+        want, tol = expected(q[rows], ks, vs, [s], [parts[s]], 0.125, True, 0)
+        close(o[rows], want, tol)
+    u = HALF_STEP[dtype]
+    off = (again.double() - without[300:300 + new].double())[:, :, rest].abs()
+    assert bool((off <= 2 * u * again[:, :, rest].double().abs() + 2 * (u + 2 ** -20 + n * 2.0 ** -24)).all())
+    for t in range(0, new, 157):
+        want, tol = expected(q[300 + t:301 + t], [ks[1][:, :n - new + t + 1]], [vs[1][:, :n - new + t + 1]], [0], [1], 0.125, True, 0)
+        close(again[t:t + 1, :, rest], want[:, :, rest], tol[:, :, rest])
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_large_scores(dtype, d):
