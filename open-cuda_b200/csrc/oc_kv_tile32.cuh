@@ -44,94 +44,126 @@ struct KvTile32Shared {
   KvJob ring[kJobs];
   float icq[2][128];              // 1 / c_q per query row, by the piece's parity
   alignas(16) float ick[2][128];  // 1 / c_k per key row, with the sign of the scale, by the tile's parity (read four at a time)
-  float icv[2];            // 1 / c_v of the V tile
-  float vpart[2][kFaConv]; // converter warps' max |v|
-  uint32_t rough[2];       // by the piece's parity: its number + 1 when V's rows are too uneven for its masks
+  alignas(16) float short_of[2][128];  // by the tile's parity, per key: what V's row lacks to keep its bits (kv_convert_values)
+  alignas(8) uint8_t uneven[2][8];     // by the tile's parity, per converter warp: some of its rows lack any
+  float icv[2];                        // 1 / c_v of the V tile
+  float vpart[2][kFaConv];             // converter warps' max |v|
   uint32_t tmem;
   int abort_word;
 };
-static_assert(offsetof(KvTile32Shared, ick) % 16 == 0 && alignof(KvTile32Shared) % 16 == 0, "ick is read as float4");
+static_assert(offsetof(KvTile32Shared, ick) % 16 == 0 && alignof(KvTile32Shared) % 16 == 0 && offsetof(KvTile32Shared, short_of) % 16 == 0,
+              "read as float4");
+static_assert(kFaConv == 8, "a tile's `uneven` is read as one 64-bit word");
 
 // The converter warp's 16 rows of a 128-row tile, from the offsets that its
-// lanes 0..15 hold (-1: a row of zeros): fa_convert_tile with rows anywhere.
-// `rough` (TILE, when given): set to `id` when one row is so much larger than
-// another that the common scaling leaves the smaller too few bits.  Rows that
-// see both do not mind; one that sees the smaller alone does, so this is
-// asked of tiles that some row sees in part.
-template <int D, bool TILE>
-__device__ __forceinline__ bool kv_convert_tile(const float* __restrict__ base, int64_t off, int d, bool vec, uint8_t* thi,
-                                                uint8_t* tlo, float* inv, float sign, int w, int lane, float* part,
-                                                uint64_t* vmax, uint32_t ph, volatile int* abort_flag,
-                                                uint32_t* rough = nullptr, uint32_t id = 0) {
-  constexpr int RPW = 128 / kFaConv, LPR = D / 4, RPS = 32 / LPR, NS = RPW / RPS;
-  const int q4 = lane % LPR, ro = lane / LPR;
-  float4 x[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int64_t o = __shfl_sync(0xffffffffu, off, s * RPS + ro);
-    x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (o >= 0 && 4 * q4 < d) {
-      const float* p = base + o + 4 * q4;
-      const int left = d - 4 * q4;  // zeros behind head_dim
-      if (vec)
-        x[s] = *reinterpret_cast<const float4*>(p);
-      else
-        x[s] = make_float4(p[0], left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
-    }
-  }
-  float cr[NS];
-  if constexpr (TILE) {
-    float mx = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) mx = fmaxf(mx, fa_absmax4(x[s]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) {
-      part[w] = mx;
-      mbar_arrive(vmax);
-    }
-    if (!warp_wait(vmax, ph, abort_flag)) return false;
-    float m = part[0];
-#pragma unroll
-    for (int j = 1; j < kFaConv; ++j) m = fmaxf(m, part[j]);
-    const int ce = fa_range_exp(m);
-    if (rough) {
-      bool uneven = false;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        float rm = fa_absmax4(x[s]);
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) rm = fmaxf(rm, __shfl_xor_sync(0xffffffffu, rm, o));
-        uneven |= rm > 0.0f && rm < m * 0.00390625f;
-      }
-      if (__any_sync(0xffffffffu, uneven) && lane == 0) *reinterpret_cast<volatile uint32_t*>(rough) = id;
-    }
-#pragma unroll
-    for (int s = 0; s < NS; ++s) cr[s] = exp2_int(ce);
-    if (w == 0 && lane == 0) *inv = exp2_int(-ce);
-  } else {
-    float mx[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) mx[s] = fa_absmax4(x[s]);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1)
-#pragma unroll
-      for (int s = 0; s < NS; ++s) mx[s] = fmaxf(mx[s], __shfl_xor_sync(0xffffffffu, mx[s], o));
+// lanes 0..15 hold (-1: a row of zeros): float4 q4 of row s * RPS + ro in x[s].
+template <int D>
+struct KvConvert {
+  static constexpr int RPW = 128 / kFaConv, LPR = D / 4, RPS = 32 / LPR, NS = RPW / RPS;
+  static __device__ __forceinline__ void load(const float* __restrict__ base, int64_t off, int d, bool vec, int lane, float4 (&x)[NS]) {
+    const int q4 = lane % LPR, ro = lane / LPR;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const int ce = fa_range_exp(mx[s]);
-      if (q4 == 0) inv[w * RPW + s * RPS + ro] = __fmul_rn(sign, exp2_int(-ce));
-      cr[s] = exp2_int(ce);
+      const int64_t o = __shfl_sync(0xffffffffu, off, s * RPS + ro);
+      x[s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (o >= 0 && 4 * q4 < d) {
+        const float* p = base + o + 4 * q4;
+        const int left = d - 4 * q4;  // zeros behind head_dim
+        if (vec)
+          x[s] = *reinterpret_cast<const float4*>(p);
+        else
+          x[s] = make_float4(p[0], left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+      }
     }
   }
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
+  static __device__ __forceinline__ void store(const float4& x, float c, int row, int q4, uint8_t* thi, uint8_t* tlo) {
     uint2 hi, lo;
-    fa_split4(x[s], cr[s], hi, lo);
-    const uint32_t to = fa_tile_off(w * RPW + s * RPS + ro, 4 * q4);
+    fa_split4(x, c, hi, lo);
+    const uint32_t to = fa_tile_off(row, 4 * q4);
     *reinterpret_cast<uint2*>(thi + to) = hi;
     *reinterpret_cast<uint2*>(tlo + to) = lo;
   }
+};
+
+// Rows of queries or keys, each by its own power of two c; inv: sign / c.
+template <int D>
+__device__ __forceinline__ void kv_convert_rows(const float* __restrict__ base, int64_t off, int d, bool vec, uint8_t* thi, uint8_t* tlo,
+                                                float* inv, float sign, int w, int lane) {
+  using C = KvConvert<D>;
+  const int q4 = lane % C::LPR, ro = lane / C::LPR;
+  float4 x[C::NS];
+  C::load(base, off, d, vec, lane, x);
+  float mx[C::NS];
+#pragma unroll
+  for (int s = 0; s < C::NS; ++s) mx[s] = fa_absmax4(x[s]);
+#pragma unroll
+  for (int o = C::LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int s = 0; s < C::NS; ++s) mx[s] = fmaxf(mx[s], __shfl_xor_sync(0xffffffffu, mx[s], o));
+#pragma unroll
+  for (int s = 0; s < C::NS; ++s) {
+    const int ce = fa_range_exp(mx[s]), row = w * C::RPW + s * C::RPS + ro;
+    if (q4 == 0) inv[row] = __fmul_rn(sign, exp2_int(-ce));
+    C::store(x[s], exp2_int(ce), row, q4, thi, tlo);
+  }
+}
+
+// Rows of values, all by one power of two c that puts the tile's largest into
+// [2^14, 2^15): through `part` and the barrier `vmax`.  Two f16 terms of a
+// scaled value t are off by at most 2^-24 (both in f16's subnormal steps) or
+// 2^-21 |t|, so a row whose largest is r keeps 2^-22 of it only from r c = 1/4
+// on.  short_of[key] = 1/4 - r c (0 for a row of zeros, which is exact), and
+// uneven[w] tells the softmax to ask whether the keys it weighs fall short on
+// the whole: a row of queries whose weights p have sum(p short_of) > 0 would
+// lose bits, whether it does not see the large values or gives them no weight.
+// Measured, 8 prompts of 300 to 777 tokens over contexts of 800 to 1000, 12
+// heads of 64: 126 us; with one value row in each of 2^-10 of the others 124,
+// of 2^-20 125.
+template <int D>
+__device__ __forceinline__ bool kv_convert_values(const float* __restrict__ base, int64_t off, int d, bool vec, uint8_t* thi, uint8_t* tlo,
+                                                  float* inv, int w, int lane, float* part, uint64_t* vmax, uint32_t ph, float* short_of,
+                                                  uint8_t* uneven, volatile int* abort_flag) {
+  using C = KvConvert<D>;
+  const int q4 = lane % C::LPR, ro = lane / C::LPR;
+  float4 x[C::NS];
+  C::load(base, off, d, vec, lane, x);
+  // the rows' maxima: lanes that differ in bit 1 << b of q4 halve the rows
+  // between them, so that lane q4 ends up with row (q4 & (NS - 1)) * RPS + ro
+  float mx[C::NS];
+#pragma unroll
+  for (int s = 0; s < C::NS; ++s) mx[s] = fa_absmax4(x[s]);
+#pragma unroll
+  for (int n = C::NS / 2; n > 0; n >>= 1) {
+    const bool upper = (q4 & n) != 0;
+#pragma unroll
+    for (int s = 0; s < n; ++s) {
+      const float keep = upper ? mx[s + n] : mx[s], give = upper ? mx[s] : mx[s + n];
+      mx[s] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, n));
+    }
+  }
+#pragma unroll
+  for (int o = C::NS; o < C::LPR; o <<= 1) mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+  const float row_max = mx[0];
+  float m = row_max;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) {
+    part[w] = m;
+    mbar_arrive(vmax);
+  }
+  if (!warp_wait(vmax, ph, abort_flag)) return false;
+  m = part[0];
+#pragma unroll
+  for (int j = 1; j < kFaConv; ++j) m = fmaxf(m, part[j]);
+  const int ce = fa_range_exp(m);
+  const float c = exp2_int(ce);
+  const float lacks = row_max > 0.0f ? 0.25f - row_max * c : 0.0f;
+  if (q4 < C::NS) short_of[w * C::RPW + q4 * C::RPS + ro] = lacks;
+  const bool some = __any_sync(0xffffffffu, lacks > 0.0f);
+  if (lane == 0) uneven[w] = some;
+  if (w == 0 && lane == 0) *inv = exp2_int(-ce);
+#pragma unroll
+  for (int s = 0; s < C::NS; ++s) C::store(x[s], c, w * C::RPW + s * C::RPS + ro, q4, thi, tlo);
   return true;
 }
 
@@ -182,7 +214,6 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
       mbar_init(&sh.job_empty[i], 1 + kFaConv + 4);
     }
     sh.abort_word = 0;
-    sh.rough[0] = sh.rough[1] = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -271,15 +302,10 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
       if (!ok) break;
       const int rr = it.r0 + mine, token = plan_token(a.p, rr);
       const int64_t qoff = mine < it.rows ? (int64_t)(it.s.q0 + token) * a.qs + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d : -1;
-      kv_convert_tile<D, false>(static_cast<const float*>(a.q), qoff, c.d, a.qvec, q_hi, q_lo, sh.icq[items & 1], 1.0f, w, lane, nullptr, nullptr, 0,
-                                abort_flag);
+      kv_convert_rows<D>(static_cast<const float*>(a.q), qoff, c.d, a.qvec, q_hi, q_lo, sh.icq[items & 1], 1.0f, w, lane);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
-      // keys that all rows of the item see
-      int all_lo, all_hi, unused;
-      plan_row_range(a.p, it.s, it.r0, unused, all_hi);
-      plan_row_range(a.p, it.s, it.r0 + it.rows - 1, all_lo, unused);
       int64_t next = kv_row_off(a, it.s.s, it.h, (it.tile0 + it.t0) * K::BK + mine, it.lo, it.hi);
       for (int t = it.t0; t < it.t1; ++t, ++n) {
         const uint32_t ph = n & 1u;
@@ -287,15 +313,13 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         if (t + 1 < it.t1) next = kv_row_off(a, it.s.s, it.h, (it.tile0 + t + 1) * K::BK + mine, it.lo, it.hi);
         ok = warp_wait(&sh.k_empty, ph ^ 1u, abort_flag);
         if (!ok) break;
-        kv_convert_tile<D, false>(kb, off, c.d, a.vec, k_hi, k_lo, sh.ick[ph], ksign, w, lane, nullptr, nullptr, 0, abort_flag);
+        kv_convert_rows<D>(kb, off, c.d, a.vec, k_hi, k_lo, sh.ick[ph], ksign, w, lane);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full);
-        const int first = max((it.tile0 + t) * K::BK, it.lo), last = min((it.tile0 + t + 1) * K::BK, it.hi);
-        const bool masked = first < all_lo || last > all_hi;  // (zeros stand in place of keys that no row sees)
         ok = warp_wait(&sh.v_empty, ph ^ 1u, abort_flag) &&
-             kv_convert_tile<D, true>(vb, off, c.d, a.vec, v_hi, v_lo, &sh.icv[ph], 1.0f, w, lane, sh.vpart[ph], &sh.vmax, ph, abort_flag,
-                                      masked ? &sh.rough[items & 1] : nullptr, items + 1);
+             kv_convert_values<D>(vb, off, c.d, a.vec, v_hi, v_lo, &sh.icv[ph], w, lane, sh.vpart[ph], &sh.vmax, ph, sh.short_of[ph],
+                                  sh.uneven[ph], abort_flag);
         if (!ok) break;
         fence_proxy_async_smem();
         __syncwarp();
@@ -351,6 +375,25 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         // 2^20 the rounding of 15 - m' can reach an exponent of 16, which no
         // f16 holds: such a row is not finite and computed again.)
         const float nb = new_m == -INFINITY ? 0.0f : __fsub_rn(15.0f, new_m);
+        // V's factors are there: whether its terms are enough for this row
+        // (kv_convert_values; the weights once more, in tiles that ask for it)
+        ok = warp_wait(&sh.v_full, ph, abort_flag);
+        if (!ok) break;
+        bool lossy = false;
+        if (*reinterpret_cast<const volatile uint64_t*>(sh.uneven[ph])) {
+          float lacks = 0.0f;
+#pragma unroll 1
+          for (int cb = 0; cb < 4; ++cb) {
+            uint32_t r[32];
+            tmem_ld32(lanes + K::S_COL + cb * 32, r);
+            tmem_ld_wait();
+            if (!all) kv_mask_chunk(r, from - cb * 32, to - cb * 32, unseen);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              lacks = fmaf(fa_ex2(__fmaf_rn(__fmul_rn(__uint_as_float(r[j]), ik[cb * 32 + j]), rq2, nb)), sh.short_of[ph][cb * 32 + j], lacks);
+          }
+          lossy = lacks > 0.0f;
+        }
         float psum = 0.0f;
 #pragma unroll 1
         for (int cb = 0; cb < 4; ++cb) {
@@ -370,6 +413,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&sh.p_full);
         l_i = __fmaf_rn(l_i, corr, psum);
         m_i = new_m;
+        if (lossy) l_i = NAN;  // and stays so: the row is computed again
         // O' of this tile -> o = o * corr + O' / c_v
         ok = warp_wait(&sh.o_full, ph, abort_flag);
         if (!ok) break;
@@ -393,15 +437,15 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&sh.o_empty);
       }
       if (!ok) break;
-      const bool whole = t0 == 0 && t1 == it.units, rough = *reinterpret_cast<volatile uint32_t*>(&sh.rough[items & 1]) == items + 1;
+      const bool whole = t0 == 0 && t1 == it.units;
       const int rr = it.r0 + row, token = plan_token(a.p, rr);
-      const float inv = rough ? NAN : l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
+      const float inv = l_i == 0.0f ? 0.0f : __fdiv_rn(1.0f, l_i);
       float* dst = whole ? static_cast<float*>(a.out) + (int64_t)(it.s.q0 + token) * a.os + (int64_t)(it.h * a.p.group + rr - token * a.p.group) * c.d
                          : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D) + plan_slot_o(K::ROWS) + (size_t)row * D;
       const bool vec = !whole || a.ovec16;
       if (!whole && row < it.rows) {
         float* slot = plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, D);
-        slot[row] = m_i, slot[K::ROWS + row] = rough ? NAN : l_i;  // the merge computes such rows again
+        slot[row] = m_i, slot[K::ROWS + row] = l_i;
       }
 #pragma unroll 1
       for (int cb = 0; cb < D / 32; ++cb) {

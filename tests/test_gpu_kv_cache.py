@@ -321,6 +321,62 @@ def test_f32_values_of_very_different_size(d, new, n):
     close(o, want, tol)
 
 
+def with_values(c, vs, s, at, rows):
+    """Puts [hk, m, d] values in place of sequence s's from token `at` on."""
+    page = c.page_size
+    for j in range(rows.shape[1]):
+        number = int(c.page_table[s, (at + j) // page])
+        c.v[0, number, :, (at + j) % page] = rows[:, j].to(c.dtype)
+    vs[s][:, at:at + rows.shape[1]] = rows.to(c.dtype)
+
+
+def two_term_tol(q, ks, vs, ids, new, scale, tol):
+    """What expected() allows, and what carrying values as two f16 terms of one
+    scaling a tile may cost.  The tile's largest is scaled into [2^14, 2^15), so
+    a scaled value t is off by half a step of f16's subnormals in each term,
+    2^-24, or by 2^-21 |t|.  A row of queries is computed on them when its
+    weights p have sum(p (1/4 - r c)) <= 0, r the largest |v| of a key and c the
+    scaling: sum(p 2^-24) <= 2^-22 sum(p r c), so any feature is off by at most
+    2^-22 times the weighted mean of the keys' largest |v|.  expected() has
+    3 * 2^-22 of the weighted mean of the feature's own |v|, which the second
+    case (2^-21) takes; a feature that is far below its row's largest needs
+    the first."""
+    largest, _ = expected(q, ks, [v.abs().amax(-1, keepdim=True).expand(v.shape) for v in vs], ids, new, scale, True, 0)
+    return tol + 2.0 ** -22 * largest
+
+
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("new, n", [(200, 260), (260, 260), (130, 3000)])
+def test_f32_large_values_of_small_weight(d, new, n):
+    """Rows that see a value of 1e12 with a weight of e^-60 beside values near 1."""
+    c, ks, vs = filled(F32, 2, d, 16, [n])
+    at = n - new + 3
+    with_values(c, vs, 0, at, 1e12 * vs[0][:, at:at + 1])
+    number = int(c.page_table[0, at // 16])
+    ks[0][:, at] = -120.0 / d
+    c.k[0, number, :, at % 16] = -120.0 / d
+    q = 0.02 * torch.randn(new, 4, d, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") + 0.5
+    o = attend(c, q, [0], [new], scale=1.0)
+    want, tol = expected(q, ks, vs, [0], [new], 1.0, True, 0)
+    close(o, want, two_term_tol(q, ks, vs, [0], [new], 1.0, tol))
+    c.check()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [7, 12, 15, 17, 18, 24, 40, 70])
+@pytest.mark.parametrize("tiny", [1, 5, 127, 128, 150])
+def test_f32_first_values_are_small(d, bits, tiny):
+    """The first tokens' values are 2^-bits of the others': the rows that see
+    them alone, the ones that see both, and another sequence beside."""
+    c, ks, vs = filled(F32, 2, d, 16, [300, 70], seed=bits)
+    with_values(c, vs, 0, 0, vs[0][:, :tiny] * 2.0 ** -bits)
+    q = torch.randn(370, 4, d, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    o = attend(c, q, [0, 1], [300, 70])
+    want, tol = expected(q, ks, vs, [0, 1], [300, 70], 1 / math.sqrt(d), True, 0)
+    close(o, want, two_term_tol(q, ks, vs, [0, 1], [300, 70], 1 / math.sqrt(d), tol))
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_nonfinite_values_that_are_seen(dtype):
     c, ks, vs = filled(dtype, 1, 64, 16, [300])
