@@ -16,7 +16,8 @@
 //   O += P V    two m16n8k16 per 16 features (V read with ldmatrix.trans),
 //               once with P rounded to the type and once with what the
 //               rounding left (p - round(p)), so that the weights carry 16 or
-//               more bits: the memory-bound kernel has the issue slots, and
+//               more bits (f16: from 2^-24 of the row's largest on, 2^-40 of
+//               it below): the memory-bound kernel has the issue slots, and
 //               the result then differs from f32 arithmetic by less than its
 //               own last rounding
 // A weight of a key that a row does not see is 0, but 0 times an infinity or
@@ -74,6 +75,9 @@ struct KvMma {
   static constexpr int STAGE = 2 * L::BYTES, RING = NS * STAGE;
   static constexpr int OS = DP + 8;                       // floats of a row of partial outputs
   static constexpr bool QREG = DP <= 128 && MT == 1;      // query fragments stay in registers
+  // f16 weights times 2^15, so that 2^-39 of the largest is still half a step
+  // of f16 (at 1 it would be 2^-25, and 2^17 keys of that make 2^-8)
+  static constexpr float P_UNIT = std::is_same<T, __half>::value ? 32768.0f : 1.0f;
   static constexpr size_t SMEM = (size_t)WARPS * RING + ROWS * L::RB;
   static_assert(WARPS * ROWS * OS * 4 <= WARPS * RING, "the partial outputs take the rings' place");
   static_assert(SMEM <= 226 * 1024, "shared memory");
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float p = kv_ex2(s[t][n][2 * i2 + e] - bs);
+              const float p = kv_ex2(s[t][n][2 * i2 + e] - bs) * K::P_UNIT;
               s[t][n][2 * i2 + e] = p;
               add += p;
             }

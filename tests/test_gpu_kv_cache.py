@@ -429,6 +429,29 @@ def test_large_scores(dtype, d):
     check(dtype, 4, 2, d, 16, [700, 300], [1, 200], scale=1e-20, seed=4)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("below", [24.6, 25.5, 27.0, 30.0])
+def test_many_keys_of_small_weight(dtype, d, new, below):
+    """One key of most of the weight and a value of 0, and 100000 of 2^-below
+    of it each, which make the output; more sequences (that share the pages)
+    than blocks, so that one block takes all keys of a sequence."""
+    n, seqs = 100000, 600
+    c, ks, vs = filled(dtype, 1, d, 64, [n])
+    c = KVCache(c.k.zero_(), c.v, c.page_table[:1].expand(seqs, -1).contiguous(), torch.full((seqs,), n, dtype=torch.int32, device="cuda"), c.refcount)
+    c.v.copy_((1.0 + torch.arange(d, device="cuda") % 7).to(dtype).expand(c.v.shape))
+    ks, vs = [torch.zeros_like(ks[0])], [c.v[0, :1, 0, :1].expand(vs[0].shape).clone()]
+    dominant = torch.full((d,), 2.0 * below * math.log(2.0) / d, device="cuda").to(dtype)
+    number = int(c.page_table[0, 0])
+    c.k[0, number, :, 5], c.v[0, number, :, 5] = dominant, 0.0
+    ks[0][:, 5], vs[0][:, 5] = dominant, 0.0
+    q = torch.full((seqs * new, 2, d), 0.5, dtype=dtype, device="cuda")
+    o = attend(c, q, range(seqs), [new] * seqs, scale=1.0, causal=False)
+    want, tol = expected(q[:1], ks, vs, [0], [1], 1.0, False, 0)
+    close(o, want.expand(o.shape), tol.expand(o.shape))
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_f32_ranges(d):
     check(F32, 4, 2, d, 16, [700, 300], [1, 200], scale=1e-18, k_scale=1e18, seed=3)
