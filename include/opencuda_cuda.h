@@ -229,11 +229,14 @@ int oc_sdpa(const float *q, const float *k, const float *v, float *o, int seq_le
  * The operations run on the current device in stream order and can be captured
  * into CUDA graphs (make one eager call on the device first: it looks up the
  * kernels' limits); calls that change one cache must be ordered by the caller,
- * attention calls alone may overlap.  Contents of device arrays (ids, offsets,
- * lengths) cannot be checked by the host: a kernel that meets a bad one sets
- * a bit of *status and stays inside the arrays.  extend, fork and copy_pages
- * then change nothing at all; the others skip the entry.  (A page table that
- * the caller has broken: fork passes a bad page number on, and reports it.) */
+ * attention calls alone may overlap.  Contents of device arrays cannot be
+ * checked by the host: a kernel that meets a bad id or page number sets a bit
+ * of *status and stays inside the arrays; offsets (cu) and lengths outside
+ * their range are taken as the nearest inside it.  extend, fork and copy_pages
+ * then change nothing at all; the others skip the entry (attention gives its
+ * rows zeros).  (A page table that the caller has broken: fork passes a bad
+ * page number on, and reports it; attention takes what a bad page would hold
+ * as zeros.) */
 #define OC_KV_F32 0
 #define OC_KV_F16 1
 #define OC_KV_BF16 2

@@ -101,12 +101,15 @@ __device__ __forceinline__ int64_t plan_head_block(const KvPlan& p, const KvSeq&
 // Block-wide: all threads call it with the same arguments and leave with the
 // same cursor.  A thread sums the sequences that are its own; sequences of
 // many row blocks (a chunk of 2048 tokens has hundreds) are summed by all.
+// The CTA of index 0, which sees every entry, reports those with new tokens
+// whose id is outside the table.
 __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c, const KvBatch& bt, int index,
                                                KvPlanShared* sh, int64_t* chunk, KvCursor& cur) {
   if (bt.n == 1) {  // one sequence of few row blocks: every thread sees all there is
     const KvSeq s = kv_seq(c, bt, 0);
     const int blocks = plan_blocks(p, s);
     if (blocks == 0) return 0;
+    if (index == 0 && s.s < 0) atomicOr(c.status, kKvBadSeq);
     if (blocks <= 8) {
       int64_t head = 0;
       for (int j = 0; j < blocks; ++j) head += plan_item(p, s, j).units;
@@ -147,6 +150,7 @@ __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c,
       KvSeq s{-1, 0, 0, 0};
       if (b < bt.n) s = kv_seq(c, bt, b);
       const int blocks = plan_blocks(p, s);
+      if (index == 0 && blocks > 0 && s.s < 0) atomicOr(c.status, kKvBadSeq);
       int64_t head = 0;
       if (blocks <= kPlanSmall)
         for (int j = 0; j < blocks; ++j) head += plan_item(p, s, j).units;

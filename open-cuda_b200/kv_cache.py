@@ -245,7 +245,8 @@ class KVCache:
         q_heads, head_dim] over their sequences' pages (scale None: 1 /
         sqrt(head_dim)); causal, and the last `window` keys alone when window
         > 0.  Rows of `out` behind the last sequence stay as they are (in a new
-        tensor: unset)."""
+        tensor: unset); those of an id outside the table are zeros, and check()
+        reports it."""
         index = self._index
         if self._current_device() != index:
             with self._torch.cuda.device(index):

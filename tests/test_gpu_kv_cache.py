@@ -519,6 +519,28 @@ def test_bad_tables_and_ids_are_reported():
             torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("bad", [-1, 3, 1 << 20])
+def test_attention_reports_bad_ids(dtype, new, bad):
+    c, ks, vs = filled(dtype, 2, 64, 16, [100, 64])  # rows 0, 1 and an empty one
+    q = torch.randn(2 * new, 4, 64, device="cuda").to(dtype)
+    for ids, one in (([bad, 1], False), ([1, bad], False), ([bad], True), ([0, bad] * 300, True)):
+        rows = len(ids) * new
+        x = q.repeat(-(-rows // (2 * new)), 1, 1)[:rows]
+        o = attend(c, x, ids, [new] * len(ids), out=torch.full_like(x, 3.0), one_each=one and new == 1).view(len(ids), new, 4, 64)
+        for i in (0, 1, len(ids) - 1):
+            if i < len(ids):
+                assert bool((o[i] == 0).all()) == (ids[i] == bad)
+        with pytest.raises(ValueError, match="sequence id outside"):
+            c.check()
+    attend(c, q[:new], [bad, 1], [0, new])  # an entry without new tokens is not looked at
+    c.check()
+    c.attention(0, q[:1].repeat(4, 1, 1))  # without ids: one more entry than there are sequences
+    with pytest.raises(ValueError, match="sequence id outside"):
+        c.check()
+
+
 def test_wrong_arguments_raise():
     c, _, _ = filled(F16, 2, 64, 16, [50, 70])
     q = torch.randn(2, 4, 64, device="cuda").half()
