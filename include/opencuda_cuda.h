@@ -301,7 +301,8 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * query head h reads kv head h / (q_heads / kv_heads).  A token at position p
  * sees keys j < seq_len with j <= p when causal and j > p - window when
  * window > 0; a row that sees none gives 0, and what a row does not see has
- * no part in it, whatever it holds.  f32 accumulation and softmax statistics.
+ * no part in it, whatever it holds.  out may not overlap q (columns of one
+ * buffer are fine).  f32 accumulation and softmax statistics.
  * Sequences of few query rows per kv head (decode steps) are bound by the
  * cache's bytes and run on warp-level matrix instructions (f32: CUDA cores);
  * more rows (over 16, f32 8) of head_dim up to 128 run on the tcgen05 tensor

@@ -60,6 +60,16 @@ inline int kv_view(const oc_kv_cache* c, KvView* out) {
   return OC_OK;
 }
 
+// Whether n rows of wa bytes at a, sa apart, and n of wb at b, sb apart, share
+// memory.  Different distances: whether the ranges do.
+inline bool kv_overlap(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb, int64_t n) {
+  const int64_t x = (int64_t)reinterpret_cast<uintptr_t>(a), y = (int64_t)reinterpret_cast<uintptr_t>(b);
+  if (x + (n - 1) * sa + wa <= y || y + (n - 1) * sb + wb <= x) return false;
+  if (sa != sb) return true;
+  const int64_t by = ((y - x) % sa + sa) % sa;  // from a row of a to the next row of b
+  return by < wa || sa - by < wb;
+}
+
 __device__ __forceinline__ float kv_f32(float x) { return x; }
 __device__ __forceinline__ float kv_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float kv_f32(__nv_bfloat16 x) { return __bfloat162float(x); }

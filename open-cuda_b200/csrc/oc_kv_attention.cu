@@ -472,6 +472,7 @@ int oc_kv_attention(const oc_kv_cache* cache, int layer, int tokens, int n, cons
   const int64_t qd = (int64_t)q_heads * c.d;
   OC_REQUIRE(q_stride >= qd && out_stride >= qd, "kv_attention: a token stride is shorter than its heads");
   const size_t es = kv_esize(cache->dtype);
+  OC_REQUIRE(!kv_overlap(q, q_stride * es, qd * es, out, out_stride * es, qd * es, tokens), "kv_attention: out overlaps q");  // rows may be computed twice
   KvAttn a;
   a.c = c;
   a.bt = KvBatch{cu, seqs, n, tokens};

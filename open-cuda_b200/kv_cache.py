@@ -244,7 +244,7 @@ class KVCache:
         """softmax(scale q . K^T) V of the new tokens' queries [tokens,
         q_heads, head_dim] over their sequences' pages (scale None: 1 /
         sqrt(head_dim)); causal, and the last `window` keys alone when window
-        > 0.  Rows of `out` behind the last sequence stay as they are (in a new
+        > 0.  `out` may not overlap q.  Rows of `out` behind the last sequence stay as they are (in a new
         tensor: unset); those of an id outside the table are zeros, and check()
         reports it."""
         index = self._index

@@ -563,6 +563,19 @@ def test_wrong_arguments_raise():
         c.extend(ints([0]), ints([1, 2]))
 
 
+def test_outputs_over_the_queries_are_refused():
+    c, ks, vs = filled(F16, 2, 64, 16, [50, 70])
+    buf = torch.randn(2, 8, 64, device="cuda").half()
+    q = buf[:, :4]
+    with pytest.raises(ValueError, match="overlaps"):
+        c.attention(0, q, out=q)
+    with pytest.raises(ValueError, match="overlaps"):
+        c.attention(0, q, out=buf[:, 3:7])
+    o = c.attention(0, q, out=buf[:, 4:])
+    want, tol = expected(q, ks, vs, [0, 1], [1, 1], 0.125, True, 0)
+    close(o, want, tol)
+
+
 # ---- append -------------------------------------------------------------------------------------------------------
 
 

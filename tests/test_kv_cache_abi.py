@@ -44,10 +44,24 @@ def attention(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=5
     (dict(q=None), "NULL"), (dict(qs=511), "stride"), (dict(os_=8), "stride"), (dict(window=-1), "window"), (dict(tokens=-1, n=-1), "negative"),
     (dict(ws_bytes=0), "workspace"), (dict(ws=None, ws_bytes=1 << 30), "workspace"), (dict(ws=0x300004, ws_bytes=1 << 30), "workspace"),
     (dict(tokens=1 << 30, n=1 << 30), "too many"),
+    (dict(out=0x100000), "overlaps"), (dict(out=0x100000 + 2 * 511), "overlaps"), (dict(out=0x100000 - 2), "overlaps"),
+    (dict(out=0x100000 + 2 * 512 * 3), "overlaps"), (dict(out=0x100000 + 2 * 512, qs=1023, os_=1023), "overlaps"),
+    (dict(out=0x100000 + 2 * 600, qs=1024, os_=600), "overlaps"), (dict(tokens=1, n=1, out=0x100000 + 2), "overlaps"),
 ])
 def test_attention_refusals(args, word):
     assert attention(**args) == oc.OC_ERR_INVALID_VALUE
     assert word in oc.last_error()
+
+
+@pytest.mark.parametrize("args", [
+    dict(out=0x100000 + 2 * 512 * 4), dict(out=0x100000 - 2 * 512 * 4), dict(out=0x100000 + 2 * 512, qs=1024, os_=1024),
+    dict(out=0x100000 - 2 * 512, qs=1024, os_=1024), dict(out=0x100000 + 2 * 600, qs=1200, os_=1200),
+    dict(tokens=1, n=1, out=0x100000 + 2 * 512),
+])
+def test_outputs_beside_the_queries_pass(args):
+    """Other columns of one buffer: the next check is what refuses."""
+    assert attention(**args) == oc.OC_ERR_INVALID_VALUE
+    assert "workspace" in oc.last_error()
 
 
 def append(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=512, k=0x200000, ks=256, v=0x300000, vs=256, qo=0x400000, qos=512,
