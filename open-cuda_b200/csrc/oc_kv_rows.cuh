@@ -10,11 +10,9 @@
 // half warp keeps a softmax of its own (running maximum and sum, log2 units),
 // four keys at a time.  The halves and warps meet in shared memory at the end
 // of an item.  A key that a row does not see is left out by a predicate, not
-// by a zero weight, so what it holds cannot reach the row.  Weights are kept
-// at 2^-24 or less (the running maximum is held 24 higher), so that the sums
-// of 2^24 values near the type's largest stay finite: a second look at lost
-// rows, as the other kernels take it, would cost this one its registers (168
-// -> 238 a thread, 14 % slower).
+// by a zero weight, so what it holds cannot reach the row.  Sums of values
+// near the type's largest may overflow: rows that do are computed again
+// (kv_row_exact).
 #pragma once
 #include "oc_kv_plan.cuh"
 
@@ -245,6 +243,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
   };
   const T* kb = static_cast<const T*>(c.k) + a.layer_off;
   const T* vb = static_cast<const T*>(c.v) + a.layer_off;
+  bool lost = false;  // a result of this thread's is not finite
 
   while (left > 0) {
     const KvItem& it = cur.it;
@@ -297,7 +296,10 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
       const uint8_t* sk = ring + (i % NS) * K::STAGE;
       const uint8_t* sv = sk + L::BYTES;
       const int kbase = (it.tile0 + t0 + i) * K::BK + warp * 16 + hw;
-#pragma unroll
+      // (unrolled, the two halves are 20 KB of code at 4 rows of 128 f32
+      // features, which the warps, each at its own place, wait for: 1 token over
+      // 20000 keys, 32 heads over 8, 72 us against 76 to 83 with the placement)
+#pragma unroll 1
       for (int k0 = 0; k0 < 16; k0 += 8) {
         float s[4][ROWS];
         uint32_t seen[4];
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           const float mx = fmaxf(fmaxf(s[0][r], s[1][r]), fmaxf(s[2][r], s[3][r]));
-          const float mn = fmaxf(m[r], mx + 24.0f), base = mn == -INFINITY ? 0.0f : mn;
+          const float mn = fmaxf(m[r], mx), base = mn == -INFINITY ? 0.0f : mn;
           const float corr = exp2f(m[r] - base);
           m[r] = mn;
           float add = 0.0f;
@@ -401,9 +403,12 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
       }
       if (whole) {
         const int rr = it.r0 + r;
-        if (e < d)
+        if (e < d) {
+          const float y = ls == 0.0f ? 0.0f : os / ls;
           static_cast<T*>(a.out)[(int64_t)(cur.s.q0 + plan_token(a.p, rr)) * a.os + (int64_t)(cur.h * g + rr - plan_token(a.p, rr) * g) * d + e] =
-              kv_from<T>(ls == 0.0f ? 0.0f : os / ls);
+              kv_from<T>(y);
+          lost |= kv_lost<T>(y);
+        }
       } else {
         if (e == 0) slot[r] = mm, slot[ROWS + r] = ls;
         slot[plan_slot_o(ROWS) + (size_t)r * DP + e] = os;
@@ -414,6 +419,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }
+  plan_lost(a, lost);
 }
 
 }  // namespace oc

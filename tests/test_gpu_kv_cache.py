@@ -252,6 +252,26 @@ def test_values_near_the_largest(dtype, big, hq, hk, d, lens, new):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hq, hk, d", [(1, 1, 64), (8, 2, 128), (4, 2, 256), (3, 1, 17), (40, 1, 64)])
+@pytest.mark.parametrize("small", [2.0 ** -100, 2.0 ** -112])
+@pytest.mark.parametrize("new", [1, 70])
+def test_values_near_the_smallest(dtype, hq, hk, d, small, new):
+    """Sums that f32 holds with all their bits: what is rounded to a subnormal,
+    at most 2^-150 at a time, is below 2^-38 of every value's size."""
+    c, ks, vs = filled(dtype, hk, d, 16, [40, 900], seed=d)
+    c.v.copy_((c.v.double() * small).to(dtype))
+    vs = [(x.double() * small).to(dtype) for x in vs]
+    q = torch.randn(1 + new, hq, d, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(dtype)
+    o = attend(c, q, [0, 1], [1, new])
+    want, tol = expected(q, ks, vs, [0, 1], [1, new], 1 / math.sqrt(d), True, 0)
+    if dtype == F32:
+        tol = two_term_tol(q, ks, vs, [0, 1], [1, new], 1 / math.sqrt(d), tol)
+    tol = tol - SMALLEST[dtype] + 940 * 2.0 ** -150
+    close(o.double() / small, want / small, tol / small)
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 80, 128])
 @pytest.mark.parametrize("new", [[1, 1], [1, 90], [90, 200]])
