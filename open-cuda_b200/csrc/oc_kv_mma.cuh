@@ -114,7 +114,6 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
   const uint32_t v_off = (uint32_t)((((lane >> 3) & 1) * 8 + (lane & 7)) * L::RB + (lane >> 4) * 16);
   const uint32_t q_off = (uint32_t)((lane & 15) * L::RB + (lane >> 4) * 16);
 
-  bool lost = false;  // a result of this thread's is not finite
   while (left > 0) {
     const KvItem& it = cur.it;
     const int t0 = cur.at, t1 = (int)min((int64_t)it.units, t0 + left);
@@ -303,6 +302,7 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
       }
     __syncthreads();
     float* slot = whole ? nullptr : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, DP);
+    bool lost = false;  // a result of this thread's is not finite
     for (int x = threadIdx.x; x < it.rows * (DP / 2); x += K::THREADS) {
       const int r = x / (DP / 2), e = x % (DP / 2) * 2;
       float mm = pm[0][r];
@@ -338,12 +338,11 @@ __global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_mma_kernel(const __gri
         *reinterpret_cast<float2*>(slot + plan_slot_o(ROWS) + (size_t)r * DP + e) = os;
       }
     }
-    __syncthreads();
+    if (__syncthreads_or(lost) && threadIdx.x == 0) plan_lost(a);
     if (t0 == 0 && !whole && threadIdx.x == 0) plan_cut(a, cur, it.units - t1, chunk);
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }
-  plan_lost(a, lost);
 }
 
 }  // namespace oc

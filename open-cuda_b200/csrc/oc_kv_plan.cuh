@@ -236,8 +236,8 @@ __device__ __forceinline__ bool plan_next(const KvPlan& p, const KvView& c, cons
 // What the cut behind a CTA's run goes through, and whether a result of the
 // run's whole items is not finite, for the merge kernel.
 struct KvCut {
-  int pieces;  // 0: nothing
-  int b, h, r0, rows, q0, lost, unused;
+  int pieces, lost;  // (read as a pair) 0: nothing
+  int b, h, r0, rows, q0, unused;
 };
 
 // Partial results of CTA `cta`, slot 0 or 1: m [br], l [br], o [br][dp]
@@ -276,14 +276,28 @@ __device__ __forceinline__ void plan_no_cut(const KvAttn& a) {
 }
 // The last item of its run began there and goes on: rest = its units behind the run.
 __device__ __forceinline__ void plan_cut(const KvAttn& a, const KvCursor& cur, int rest, int64_t chunk) {
-  reinterpret_cast<KvCut*>(a.ws)[blockIdx.x] =
-      KvCut{2 + (int)((rest - 1) / chunk), cur.b, cur.h, cur.it.r0, cur.it.rows, cur.s.q0, 0, 0};
+  KvCut& cut = reinterpret_cast<KvCut*>(a.ws)[blockIdx.x];
+  cut.b = cur.b, cut.h = cur.h, cut.r0 = cur.it.r0, cut.rows = cur.it.rows, cut.q0 = cur.s.q0;
+  cut.pieces = 2 + (int)((rest - 1) / chunk);
 }
-// All threads, the last to write there: `lost` of any of them.  Such rows are
-// computed again by the merge kernel: it has no waits that would run out, and
-// the whole GPU for them.
-__device__ __forceinline__ void plan_lost(const KvAttn& a, bool lost) {
-  if (__syncthreads_or(lost) && threadIdx.x == 0) reinterpret_cast<KvCut*>(a.ws)[blockIdx.x].lost = 1;
-}
+// One thread: a result of the run's whole items is not finite.
+__device__ __forceinline__ void plan_lost(const KvAttn& a) { reinterpret_cast<KvCut*>(a.ws)[blockIdx.x].lost = 1; }
+
+constexpr int kMostCtas = 2048;  // of an attention kernel's grid
+
+// The partial results of one launch.
+struct KvPart {
+  float* ws;
+  int ctas, br, groups, dp;  // groups: of R rows, that an item can have; dp: floats of a row
+  KvPlan p;
+};
+struct KvParts {
+  KvPart of[2];
+  int count;
+};
+
+// Joins the partial results of a call's launches, and computes again what they
+// lost (oc_kv_merge.cu).  few: one row of an item at a time; dp: the widest.
+int kv_merge(const KvAttn& a, const KvParts& parts, int dtype, bool few, int dp, int grid, cudaStream_t s);
 
 }  // namespace oc

@@ -61,102 +61,6 @@ __device__ __forceinline__ bool kv_lost(float y) {
   return !isfinite(y);
 }
 
-// One row of one query head from the definition, by all threads of a block
-// (whole warps): for rows whose result was lost.  Reads only keys that the row
-// sees, each once: a warp takes 32 of them at a time and keeps what it has so
-// far divided by the sum so far, so that values near the type's largest do not
-// overflow (the fast kernels divide at the end); the warps meet in `sh`
-// (kv_exact_floats).
-template <typename T, int DP>
-__device__ __noinline__ void kv_row_exact(const KvAttn& a, KvSeq s, int h, int row, float* sh) {
-  const KvView& c = a.c;
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = c.d, g = a.p.group;
-  const int64_t token = s.q0 + row / g, head = (int64_t)(h * g + row % g) * d;
-  const T* q = static_cast<const T*>(a.q) + token * a.qs + head;
-  const T* kb = static_cast<const T*>(c.k) + a.layer_off;
-  const T* vb = static_cast<const T*>(c.v) + a.layer_off;
-  int lo, hi;
-  plan_row_range(a.p, s, row, lo, hi);
-  constexpr int NF = DP / 32, U = 2;  // features a lane, keys in flight
-  float x[NF], o[NF] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NF; ++i) x[i] = lane + 32 * i < d ? kv_f32(q[lane + 32 * i]) : 0.0f;
-  for (int64_t key0 = lo + 32 * (int64_t)warp; key0 < hi; key0 += 32 * warps) {
-    const int n = (int)min((int64_t)32, hi - key0);
-    const int64_t off = kv_row_off(a, s.s, h, (int)(key0 + min(lane, n - 1)), lo, hi);  // -1: a bad page, keys and values of zero
-    float score = -INFINITY;
-    for (int j0 = 0; j0 < n; j0 += U) {
-      float dot[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t at = __shfl_sync(0xffffffffu, off, min(j0 + u, n - 1));
-        dot[u] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NF; ++i)
-          if (lane + 32 * i < d && at >= 0) dot[u] = fmaf(x[i], kv_f32(kb[at + lane + 32 * i]), dot[u]);
-      }
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1)
-#pragma unroll
-        for (int u = 0; u < U; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], w);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (lane == j0 + u && lane < n) score = dot[u] * a.scale2;
-    }
-    float mn = score;
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
-    mn = fmaxf(m, mn);
-    const float base = mn == -INFINITY ? 0.0f : mn, p = lane < n ? exp2f(score - base) : 0.0f;
-    float ln = p;
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) ln += __shfl_xor_sync(0xffffffffu, ln, w);
-    const float before = l * exp2f(m - base);
-    l = before + ln;
-    m = mn;
-    const float keep = l == 0.0f ? 0.0f : before / l, weight = l == 0.0f ? 0.0f : p / l;
-#pragma unroll
-    for (int i = 0; i < NF; ++i) o[i] *= keep;
-#pragma unroll 2
-    for (int j = 0; j < n; ++j) {
-      const int64_t at = __shfl_sync(0xffffffffu, off, j);
-      const float w = __shfl_sync(0xffffffffu, weight, j);
-#pragma unroll
-      for (int i = 0; i < NF; ++i)
-        if (lane + 32 * i < d && at >= 0) o[i] = fmaf(w, kv_f32(vb[at + lane + 32 * i]), o[i]);
-    }
-  }
-  float *ms = sh + warps * d, *ls = ms + warps;
-#pragma unroll
-  for (int i = 0; i < NF; ++i)
-    if (lane + 32 * i < d) sh[warp * d + lane + 32 * i] = o[i];
-  if (lane == 0) ms[warp] = m, ls[warp] = l;
-  __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < warps; ++w) top = fmaxf(top, ms[w]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  for (int w = 0; w < warps; ++w) sum = fmaf(ls[w], exp2f(ms[w] - base), sum);
-  T* out = static_cast<T*>(a.out) + token * a.os + head;
-  for (int e = threadIdx.x; e < d; e += blockDim.x) {
-    float y = 0.0f;
-    for (int w = 0; w < warps; ++w) y = fmaf(ls[w] * exp2f(ms[w] - base) / sum, sh[w * d + e], y);
-    out[e] = kv_from<T>(sum == 0.0f ? 0.0f : y);
-  }
-  __syncthreads();
-}
-// Floats of `sh` for d features.
-constexpr int kv_exact_floats(int threads, int d) { return threads / 32 * (d + 2); }
-
-// Whether the row holds a result that is not finite.
-template <typename T>
-__device__ __forceinline__ bool kv_row_lost(const KvAttn& a, const KvSeq& s, int h, int row, int first, int step) {
-  const int g = a.p.group, d = a.c.d;
-  const T* out = static_cast<const T*>(a.out) + (int64_t)(s.q0 + row / g) * a.os + (int64_t)(h * g + row % g) * d;
-  bool lost = false;
-  for (int e = first; e < d; e += step) lost |= !isfinite(kv_f32(out[e]));
-  return lost;
-}
-
 // Requests the 16 rows whose offsets lanes 0..15 (and 16..31 again) hold.
 template <typename T, int DP>
 __device__ __forceinline__ void kv_load_tile(const KvAttn& a, const T* kb, const T* vb, int64_t off, uint8_t* sk,
@@ -243,7 +147,6 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
   };
   const T* kb = static_cast<const T*>(c.k) + a.layer_off;
   const T* vb = static_cast<const T*>(c.v) + a.layer_off;
-  bool lost = false;  // a result of this thread's is not finite
 
   while (left > 0) {
     const KvItem& it = cur.it;
@@ -388,6 +291,7 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
     }
     __syncthreads();
     float* slot = whole ? nullptr : plan_slot(a, blockIdx.x, t0 == 0 ? 1 : 0, DP);
+    bool lost = false;  // a result of this thread's is not finite
     for (int x = threadIdx.x; x < it.rows * DP; x += K::THREADS) {
       const int r = x / DP, e = x % DP;
       float mm = pm[0][r];
@@ -414,12 +318,11 @@ __global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_consta
         slot[plan_slot_o(ROWS) + (size_t)r * DP + e] = os;
       }
     }
-    __syncthreads();
+    if (__syncthreads_or(lost) && threadIdx.x == 0) plan_lost(a);
     if (t0 == 0 && !whole && threadIdx.x == 0) plan_cut(a, cur, it.units - t1, chunk);
     left -= t1 - t0;
     if (left > 0) plan_next(a.p, c, a.bt, cur);
   }
-  plan_lost(a, lost);
 }
 
 }  // namespace oc

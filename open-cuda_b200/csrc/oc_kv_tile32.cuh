@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(K::THREADS, 1) kv_tile32_kernel(const __grid_c
     if (!ok) kernel_fail(a.dev_status, abort_flag, kDevTimeoutProducer);
   }
   tc_fence_before();
-  plan_lost(a, lost);
+  if (__syncthreads_or(lost) && threadIdx.x == 0) plan_lost(a);
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, K::TMEM_COLS);
