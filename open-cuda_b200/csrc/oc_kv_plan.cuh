@@ -214,18 +214,27 @@ __device__ __forceinline__ int64_t plan_locate(const KvPlan& p, const KvView& c,
   return total;
 }
 
-// The next item's first unit; false at the end of the list.
+// The next item's first unit; false at the end of the list.  Whole warps.
 __device__ __forceinline__ bool plan_next(const KvPlan& p, const KvView& c, const KvBatch& bt, KvCursor& cur) {
   cur.at = 0;
   if (++cur.j >= cur.blocks) {
     cur.j = 0;
     if (++cur.h >= c.hk) {
       cur.h = 0;
-      for (;;) {
-        if (++cur.b >= bt.n) return false;
-        cur.s = kv_seq(c, bt, cur.b);
-        cur.blocks = plan_blocks(p, cur.s);
-        if (cur.blocks > 0) break;
+      // 32 entries at a time: thousands of the other class may lie between
+      const int lane = threadIdx.x & 31;
+      if (++cur.b >= bt.n) return false;
+      cur.s = kv_seq(c, bt, cur.b);
+      cur.blocks = plan_blocks(p, cur.s);
+      for (int b0 = cur.b + 1; cur.blocks == 0; b0 += 32) {
+        if (b0 >= bt.n) return false;
+        const int b = b0 + lane;
+        const uint32_t some = __ballot_sync(0xffffffffu, b < bt.n && plan_blocks(p, kv_seq(c, bt, b)) > 0);
+        if (some) {
+          cur.b = b0 + __ffs(some) - 1;
+          cur.s = kv_seq(c, bt, cur.b);
+          cur.blocks = plan_blocks(p, cur.s);
+        }
       }
     }
   }

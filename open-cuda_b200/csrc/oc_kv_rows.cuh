@@ -114,12 +114,13 @@ struct KvRows {
   static constexpr int NV = (L::CHUNKS + 15) / 16;  // 16-byte chunks of a row per lane
   static constexpr int F = NV * VN;                 // features per lane
   static constexpr size_t SMEM = (size_t)WARPS * RING;
+  static constexpr int FIT = (int)(224 * 1024 / (SMEM + 1024)), CTAS = FIT < 3 ? FIT : 3;  // an SM: what shared memory and registers allow
   static_assert(PARTS * ROWS * DP * 4 <= WARPS * RING, "the partial outputs take the rings' place");
   static_assert(SMEM <= 226 * 1024, "shared memory");
 };
 
 template <typename K>
-__global__ void __launch_bounds__(K::THREADS) kv_rows_kernel(const __grid_constant__ KvAttn a) {
+__global__ void __launch_bounds__(K::THREADS, K::CTAS) kv_rows_kernel(const __grid_constant__ KvAttn a) {
   using T = typename K::T;
   using L = typename K::L;
   constexpr int ROWS = K::ROWS, F = K::F, NV = K::NV, VN = K::VN, NS = K::NS, DP = K::DP;

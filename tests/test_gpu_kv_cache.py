@@ -190,6 +190,21 @@ def test_many_short_sequences(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("apart", [31, 32, 2500])
+def test_chunks_far_apart_in_the_batch(dtype, apart):
+    """Chunks of dozens of row blocks with single tokens and entries without
+    any between them, more than a block has threads."""
+    lens = [900] + [1 + i % 9 for i in range(apart)] + [40, 1200, 33]
+    new = [700] + [int(i % 3 > 0) for i in range(apart)] + [0, 650, 30]
+    c, ks, vs = filled(dtype, 1, 64, 16, lens, seed=apart)
+    q = torch.randn(sum(new), 16, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    o = attend(c, q, range(len(lens)), new)
+    want, tol = expected(q, ks, vs, range(len(lens)), new, 0.125, True, 0)
+    close(o, want, tol)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("new", [1, 3, 70])
 def test_one_long_sequence_is_split(dtype, new):
     c, q, o = check(dtype, 8, 2, 128, 64, [40000], [new], seed=new)
