@@ -309,7 +309,8 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * cores, f32 as pairs of f16 terms (f16 and bf16: 16-byte-aligned rows).
  * workspace: oc_kv_attention_workspace_size bytes, for partial results of
  * long sequences that several blocks share; calls that may overlap need one
- * each. */
+ * each, and so do calls of several host threads on one stream (a call is two
+ * or three kernels). */
 int oc_kv_attention_workspace_size(const oc_kv_cache *cache, int tokens, int n, int q_heads, size_t *bytes);
 int oc_kv_attention(const oc_kv_cache *cache, int layer, int tokens, int n, const int32_t *cu, const int32_t *seqs,
                     int q_heads, const void *q, int64_t q_stride, void *out, int64_t out_stride, float scale,

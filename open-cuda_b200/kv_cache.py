@@ -18,13 +18,14 @@ can be captured into a CUDA graph.
 `seqs`, `counts`, `cu`, ... are int32 CUDA tensors: entry b of a batch is
 sequence seqs[b] (seqs None: b) with new tokens cu[b] .. cu[b + 1] - 1 (cu
 None: one token each).  Calls on one cache are ordered by the caller (one
-stream, or events); attention alone may run on several streams at once
-(threads that use one stream take turns: its calls share a workspace).
+stream, or events); attention alone may run on several streams and from
+several threads at once.
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import opencuda_cuda as oc
 
@@ -83,7 +84,7 @@ class KVCache:
         self._capturing, self._empty_like, self._scale = torch.cuda.is_current_stream_capturing, torch.empty_like, 1.0 / math.sqrt(dim)
         self._append, self._attention, self._extend, self._fork = lib.oc_kv_append, lib.oc_kv_attention, lib.oc_kv_extend, lib.oc_kv_fork
         self._free, self._compact, self._copy = lib.oc_kv_free, lib.oc_kv_compact, lib.oc_kv_copy_pages
-        self._ws_bytes, self._workspaces = {}, {}
+        self._ws_bytes, self._workspaces, self._turn = {}, {}, threading.Lock()
         ws = oc.sz(0)
         oc.check(lib.oc_kv_attention_workspace_size(self._p, 0, 0, heads, C.byref(ws)))  # checks the shape as a whole
 
@@ -264,15 +265,17 @@ class KVCache:
         need = self._ws_bytes.get((tokens, n, heads)) or self._workspace_size(tokens, n, heads)
         stream = self._raw_stream(index)
         # eager calls of one stream run one after another and share a scratch
-        # buffer; a captured call gets its own, which its graph keeps
-        if self._capturing():
-            ws = self._new_bytes(need)
-        else:
-            ws = self._workspaces.get(stream)
-            if ws is None or ws.numel() < need:
-                ws = self._workspaces[stream] = self._new_bytes(need)
-        rc = self._attention(self._p, layer, tokens, n, cp, sp, heads, q.data_ptr(), qs, out.data_ptr(), os_,
-                             self._scale if scale is None else scale, 1 if causal else 0, window, ws.data_ptr(), need, stream)
+        # buffer (of several kernels each, so threads take turns here); a
+        # captured call gets its own, which its graph keeps
+        with self._turn:
+            if self._capturing():
+                ws = self._new_bytes(need)
+            else:
+                ws = self._workspaces.get(stream)
+                if ws is None or ws.numel() < need:
+                    ws = self._workspaces[stream] = self._new_bytes(need)
+            rc = self._attention(self._p, layer, tokens, n, cp, sp, heads, q.data_ptr(), qs, out.data_ptr(), os_,
+                                 self._scale if scale is None else scale, 1 if causal else 0, window, ws.data_ptr(), need, stream)
         if rc:
             oc.check(rc)
         return out

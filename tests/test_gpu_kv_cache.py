@@ -15,6 +15,7 @@ round each weight once more: eps/2 * A.  Of f32, the products may be carried
 as pairs of f16 terms (22 bits each operand): 3 * 2^-22 * S more in a score,
 3 * 2^-22 * A more in the output."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -1075,6 +1076,39 @@ def test_graphs_and_streams():
                 gg.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_threads_on_one_stream(dtype):
+    """Four threads call attention on one stream, and two on streams of their
+    own, each with a batch of its own: long sequences that many blocks share,
+    and chunks."""
+    hq, hk, d = 8, 2, 64
+    lens = [9000, 90, 5000, 700]
+    c, _, _ = filled(dtype, hk, d, 16, lens)
+    batches = [([0], [1]), ([2, 1], [1, 60]), ([3, 0], [300, 3]), ([2], [40]), ([0, 1, 2, 3], [1, 1, 1, 1]), ([3], [500])]
+    work = []
+    for i, (ids, new) in enumerate(batches):
+        q = torch.randn(sum(new), hq, d, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").to(dtype)
+        work.append((q, ints(np.concatenate([[0], np.cumsum(new)])), ints(ids)))
+    want = [c.attention(0, *w) for w in work]
+    shared = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(shared if i < 4 else torch.cuda.Stream()):
+            outs = [c.attention(0, *work[i]) for _ in range(200)]
+        torch.cuda.synchronize()
+        bad.extend(i for o in outs if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, f"{len(bad)} calls differ, of threads {sorted(set(bad))}"
     c.check()
 
 
