@@ -474,7 +474,7 @@ int oc_kv_compact(const oc_kv_cache* cache, void* stream) {
   const size_t pb = page_bytes_of(c, cache->dtype);
   OC_CHECK_CUDA(launch_pdl_ex(kv_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, c, cache->scratch));
   // at most half of the pages move; the CTAs of a layer share what does
-  const int x = std::max(1, std::min((c.pages + 1) / 2, std::max(32, 148 * 16 / (2 * c.layers))));
+  const int x = std::max(1, std::min((c.pages + 1) / 2, std::max(32, std::max(1, sm_count()) * 16 / (2 * c.layers))));
   return by_width(c, pb, [&](auto v) {
     OC_CHECK_CUDA(launch_pdl_ex(kv_compact_kernel<decltype(v)>, dim3(x, 2 * c.layers), dim3(256), 0, s, c,
                                 cache->scratch, pb));
