@@ -221,7 +221,7 @@ int oc_sdpa(const float *q, const float *k, const float *v, float *o, int seq_le
  * holds seq_len[s] tokens; token t sits in page page_table[s][t / page_size]
  * at offset t % page_size.  refcount[p] counts the sequences that hold page p
  * (0 = free); a page that two sequences share is full, so it is never
- * written.  All arrays are device memory of the caller; a fresh cache has
+ * written (append a sequence's new tokens before it is forked).  All arrays are device memory of the caller; a fresh cache has
  * page_table -1 and seq_len, refcount and status 0 (what no sequence holds is
  * never looked at, so the pools may hold anything).  page_size is a power of
  * two up to 1024, head_dim at most 256.
@@ -306,7 +306,16 @@ int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const i
  * Sequences of few query rows per kv head (decode steps) are bound by the
  * cache's bytes and run on warp-level matrix instructions (f32: CUDA cores);
  * more rows (over 16, f32 8) of head_dim up to 128 run on the tcgen05 tensor
- * cores, f32 as pairs of f16 terms (f16 and bf16: 16-byte-aligned rows).
+ * cores (f16 and bf16: 16-byte-aligned rows).  So a token's result may differ
+ * in its last bits with the batch that it came in:
+ *   f16, bf16  few rows: weights as two terms of the type (16 bits or more);
+ *              more rows: weights rounded to the type once.  An f16 weight may
+ *              be off by 2^-40, with more rows 2^-36, of the row's largest.
+ *   f32        few rows: f32.  More rows: queries, keys, values and weights as
+ *              two f16 terms each, 22 bits, or 2^-38 of the largest of the row
+ *              (values: of the 128 keys of a tile) where that is more; rows
+ *              whose weights meet values too small for that on the whole are
+ *              computed in f32.
  * workspace: oc_kv_attention_workspace_size bytes, for partial results of
  * long sequences that several blocks share; calls that may overlap need one
  * each, and so do calls of several host threads on one stream (a call is two

@@ -213,6 +213,43 @@ def test_one_long_sequence_is_split(dtype, new):
         assert torch.equal(o, attend(c, q, [0], [new]))  # the same bits each time
 
 
+def block_values(n, d, device="cuda"):
+    """[1, n, d]: feature f is 1 for the keys of the f-th of d equal blocks, 0
+    for the others, so output f is the weight of block f.  Nothing cancels: what
+    expected() allows is a fraction of that weight, and a piece of the keys that
+    is lost shows in the features of its blocks."""
+    return (torch.arange(n, device=device)[:, None] * d // n == torch.arange(d, device=device)[None, :]).double()[None]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq, hk, d", [(8, 2, 128), (4, 4, 64), (6, 2, 96), (2, 1, 256), (28, 4, 128), (3, 1, 33)])
+@pytest.mark.parametrize("new, n", [(1, 40000), (3, 40000), (70, 12000), (300, 7000)])
+@pytest.mark.parametrize("scale", [None, 1.0])
+def test_every_key_counts(dtype, hq, hk, d, new, n, scale):
+    """Long contexts in pieces, joined: none is lost, and none counts twice.
+    With a scale of 1 a few keys have the weight, and f32 queries, keys or
+    weights of fewer bits would show.
+
+    f32 tiles carry a weight as two f16 terms of 2^15 times it, the largest of
+    the row being 1: half a step of f16's subnormals in each, so 2^-24 of the
+    scaled weight, 2^-39 of the largest a key, however small the weight itself;
+    the sum that divides is at least the largest.  expected() has relative
+    errors of weights alone, so 2^-39 sum |v| is added for features that have
+    next to no weight."""
+    c, ks, vs = filled(dtype, hk, d, 64, [n, 200], seed=new)
+    rows = block_values(n, d).to(dtype).expand(hk, n, d)
+    at = torch.arange(n, device="cuda")
+    c.v[0, c.page_table[0].long()[at // 64], :, at % 64] = rows.transpose(0, 1)
+    q = torch.randn(new + 1, hq, d, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").to(dtype)
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    o = attend(c, q, [0, 1], [new, 1], scale=scale)
+    want, tol = expected(q, ks, [rows, vs[1]], [0, 1], [new, 1], scale, True, 0)
+    if dtype == F32:
+        tol[:new] += 2.0 ** -39 * rows[0].double().sum(0)
+    close(o, want, tol)
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_layers_strides_and_scales(dtype):
     c, ks, vs = filled(dtype, 2, 64, 16, [50, 130], layers=3, layer=1)
