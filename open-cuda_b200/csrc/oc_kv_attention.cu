@@ -49,8 +49,9 @@ static KvLaunch shape_of(void (*kern)(KvAttn)) {
 
 // On the CUDA cores; `rows`: the most that a sequence's kv head can have.
 // The rows of an item are the registers' and the multiply-adds' cost, used or
-// not: one token over 20000 keys, 32 f32 heads of 128 over 8, takes 75 us in
-// items of 4 rows (2.2 TB/s; multiply-adds bound it) and 153 in items of 8.
+// not: one token over 20000 keys, 32 f32 heads of 128 over 8, takes 72 us in
+// items of 4 rows (2.3 TB/s) and 153 in items of 8.  (What bounds it:
+// oc_kv_rows.cuh.)
 template <typename T>
 static KvLaunch scalar_launch(int d, int rows) {
   auto go = [](auto k) { return shape_of<decltype(k)>(kv_rows_kernel<decltype(k)>); };

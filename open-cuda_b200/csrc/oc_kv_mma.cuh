@@ -1,12 +1,12 @@
-// oc_kv_mma.cuh -- attention over the paged cache in items of 16 or 32 query
-// rows, f16 and bf16: decode steps, and chunks of head_dims that the tcgen05
-// tiles do not take.
+// oc_kv_mma.cuh -- attention over the paged cache in items of 16 query rows,
+// f16 and bf16: decode steps, and chunks that the tcgen05 tiles do not take
+// (head_dims over 128; items of 32 rows: queries that are not 16-byte aligned).
 //
 // Bound: the cache's bytes (a decode step of 8 rows does 32 flops per element
 // read).  On the CUDA cores 8 rows cost more issue slots than the memory
 // leaves (0.1 of the copy rate measured, 3.7 ms for 64 sequences of 2 to 15 k
-// keys, 32 heads of 128 over 8; here 374 us = 6.03 TB/s, 0.93), so the
-// products run on warp-level matrix instructions, whose 16 rows a decode
+// keys, 32 heads of 128 over 8; here 387 to 405 us a call among others = 5.6 to
+// 5.8 TB/s, 0.87 to 0.9), so the products run on warp-level matrix instructions, whose 16 rows a decode
 // step's query heads of one kv head fill in part; tcgen05 tiles of 128 rows
 // would be mostly empty and would put a block-wide hand-over behind every
 // tile.  A warp works alone: its own 16-key tiles, its own cp.async ring, its

@@ -17,14 +17,15 @@
 // the chain of a sub-tile (scores out of tensor memory 420 cycles, maximum
 // 370, exponentials 1500, then its two products): 3900 cycles a tile by a
 // clock record.  Measured: chunks of 1.9 to 2 k tokens over 14 to 16 k keys,
-// 32 heads of 128 over 8, 930 to 1010 us = 0.9 to 0.98 PFLOP/s.  Not kept, all
-// slower there: two threads a row (16 softmax warps, 96 registers: 1120 us),
+// 32 heads of 128 over 8, 1020 us a call = 0.89 PFLOP/s.  Not kept, all slower
+// there: two threads a row (16 softmax warps, 96 registers: 1120 us),
 // exponentials in part as polynomials on the multiply-add pipe (1060 to 1200),
 // items of 128 rows whose tiles two softmax groups take in turn (1215: twice
 // the keys' traffic).  O stays in tensor memory and is rescaled only when a row's
 // maximum has grown by more than 2^8 since the last time (f16: 2^4; larger
 // weights lose nothing): after the first tiles that is rare, so the softmax
-// almost never waits for the accumulator.
+// almost never waits for the accumulator.  (That, and the early start of the
+// product, are published ideas of attention on this generation of GPUs.)
 //
 // 384 threads, one CTA an SM:
 //   warp 0       TMEM allocator, MMA issuer (lane 0)
