@@ -289,8 +289,8 @@ int oc_kv_copy_pages(const oc_kv_cache *cache, const int32_t *src, const int32_t
  *   the first rot_dim features are rotated by position * inv_freq[j]
  *        (inv_freq [rot_dim / 2] f32, the angle in f64): pairs (j, j +
  *        rot_dim / 2), or (2j, 2j + 1) when interleaved; rot_dim 0: none.
- * q_out [tokens][q_heads][head_dim] may be q itself; q_heads 0: keys and
- * values alone.  Rows of tokens behind the last sequence stay as they are. */
+ * q_out [tokens][q_heads][head_dim] may be q itself, and overlaps nothing
+ * else; q_heads 0: keys and values alone.  Rows of tokens behind the last sequence stay as they are. */
 int oc_kv_append(const oc_kv_cache *cache, int layer, int tokens, int n, const int32_t *cu, const int32_t *seqs,
                  int q_heads, const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
                  int64_t v_stride, void *q_out, int64_t q_out_stride, const void *q_weight, const void *k_weight,

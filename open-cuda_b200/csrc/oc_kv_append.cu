@@ -450,6 +450,15 @@ extern "C" int oc_kv_append(const oc_kv_cache* cache, int layer, int tokens, int
   const int64_t kd = (int64_t)c.hk * c.d, qd = (int64_t)q_heads * c.d;
   OC_REQUIRE(k_stride >= kd && v_stride >= kd && (q_heads == 0 || (q_stride >= qd && q_out_stride >= qd)),
              "kv_append: a token stride is shorter than its heads");
+  const int64_t es = (int64_t)kv_esize(cache->dtype);
+  if (q_heads) {
+    const bool in_place = q_out == q && (q_out_stride == q_stride || tokens == 1);
+    OC_REQUIRE(in_place || !kv_overlap(q, q_stride * es, qd * es, q_out, q_out_stride * es, qd * es, tokens),
+               "kv_append: q_out overlaps q and is not q itself");
+    OC_REQUIRE(!kv_overlap(k, k_stride * es, kd * es, q_out, q_out_stride * es, qd * es, tokens) &&
+                   !kv_overlap(v, v_stride * es, kd * es, q_out, q_out_stride * es, qd * es, tokens),
+               "kv_append: q_out overlaps k or v");
+  }
   KvAppend a;
   a.c = c;
   a.bt = KvBatch{cu, seqs, n, tokens};

@@ -73,7 +73,9 @@ def append(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=512,
 @pytest.mark.parametrize("args, word", [
     (dict(layer=2), "layer"), (dict(n=3), "one token"), (dict(rot=3, inv=0x9000), "even"), (dict(rot=66, inv=0x9000), "rot_dim"),
     (dict(rot=64), "inv_freq"), (dict(k=None), "NULL"), (dict(qo=None), "NULL"), (dict(ks=255), "stride"), (dict(qs=511), "stride"),
-    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"), (dict(heads=1 << 26, qs=1 << 33, qos=1 << 33), "too many heads"),
+    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"),
+    (dict(qo=0x100002), "overlaps q"), (dict(qo=0x100000, qos=1024), "overlaps q"), (dict(qo=0x200000), "overlaps k or v"),
+    (dict(qo=0x300000 + 2 * 255), "overlaps k or v"), (dict(qo=0x200000 - 2 * 512, qos=512 + 256, ks=512 + 256, k=0x200000 - 2), "overlaps k or v"), (dict(heads=1 << 26, qs=1 << 33, qos=1 << 33), "too many heads"),
 ])
 def test_append_refusals(args, word):
     assert append(**args) == oc.OC_ERR_INVALID_VALUE
