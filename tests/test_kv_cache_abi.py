@@ -44,13 +44,19 @@ def attention(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=5
     (dict(q=None), "NULL"), (dict(qs=511), "stride"), (dict(os_=8), "stride"), (dict(window=-1), "window"), (dict(tokens=-1, n=-1), "negative"),
     (dict(ws_bytes=0), "workspace"), (dict(ws=None, ws_bytes=1 << 30), "workspace"), (dict(ws=0x300004, ws_bytes=1 << 30), "workspace"),
     (dict(tokens=1 << 30, n=1 << 30), "too many"),
-    (dict(out=0x100000), "overlaps"), (dict(out=0x100000 + 2 * 511), "overlaps"), (dict(out=0x100000 - 2), "overlaps"),
-    (dict(out=0x100000 + 2 * 512 * 3), "overlaps"), (dict(out=0x100000 + 2 * 512, qs=1023, os_=1023), "overlaps"),
-    (dict(out=0x100000 + 2 * 600, qs=1024, os_=600), "overlaps"), (dict(tokens=1, n=1, out=0x100000 + 2), "overlaps"),
 ])
 def test_attention_refusals(args, word):
     assert attention(**args) == oc.OC_ERR_INVALID_VALUE
     assert word in oc.last_error()
+
+
+@pytest.mark.parametrize("args", [
+    dict(out=0x100000), dict(out=0x100000 + 2 * 511), dict(out=0x100000 - 2), dict(out=0x100000 + 2 * 512 * 3),
+    dict(out=0x100000 + 2 * 512, qs=1023, os_=1023), dict(out=0x100000 + 2 * 600, qs=1024, os_=600), dict(tokens=1, n=1, out=0x100000 + 2),
+])
+def test_outputs_over_the_queries_are_refused(args):
+    assert attention(**args) == oc.OC_ERR_INVALID_VALUE
+    assert "overlaps" in oc.last_error()
 
 
 @pytest.mark.parametrize("args", [
@@ -73,11 +79,18 @@ def append(c=None, layer=0, tokens=4, n=4, cu=None, heads=8, q=0x100000, qs=512,
 @pytest.mark.parametrize("args, word", [
     (dict(layer=2), "layer"), (dict(n=3), "one token"), (dict(rot=3, inv=0x9000), "even"), (dict(rot=66, inv=0x9000), "rot_dim"),
     (dict(rot=64), "inv_freq"), (dict(k=None), "NULL"), (dict(qo=None), "NULL"), (dict(ks=255), "stride"), (dict(qs=511), "stride"),
-    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"),
-    (dict(qo=0x100002), "overlaps q"), (dict(qo=0x100000, qos=1024), "overlaps q"), (dict(qo=0x200000), "overlaps k or v"),
-    (dict(qo=0x300000 + 2 * 255), "overlaps k or v"), (dict(qo=0x200000 - 2 * 512, qos=512 + 256, ks=512 + 256, k=0x200000 - 2), "overlaps k or v"), (dict(heads=1 << 26, qs=1 << 33, qos=1 << 33), "too many heads"),
+    (dict(tokens=5, n=5), "more entries"), (dict(heads=-1), "negative"), (dict(heads=1 << 26, qs=1 << 33, qos=1 << 33), "too many heads"),
 ])
 def test_append_refusals(args, word):
+    assert append(**args) == oc.OC_ERR_INVALID_VALUE
+    assert word in oc.last_error()
+
+
+@pytest.mark.parametrize("args, word", [
+    (dict(qo=0x100002), "overlaps q"), (dict(qo=0x100000, qos=1024), "overlaps q"), (dict(qo=0x200000), "overlaps k or v"),
+    (dict(qo=0x300000 + 2 * 255), "overlaps k or v"), (dict(qo=0x200000 - 2 * 512, qos=512 + 256, ks=512 + 256, k=0x200000 - 2), "overlaps k or v"),
+])
+def test_append_over_its_inputs_is_refused(args, word):
     assert append(**args) == oc.OC_ERR_INVALID_VALUE
     assert word in oc.last_error()
 
